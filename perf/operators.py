@@ -118,7 +118,7 @@ def work(case):
         n, (lens, news) = case["n_req"], _lens(case)
         rows = sum(news)
         words = -(-case["new"] // 64)
-        return {"bytes": 2 * 4 * n * case["width"] + 6 * 4 * n + rows * (4 + 4 + 8 + (4 + 8 * words)), "flops": 0}
+        return {"bytes": 2 * 4 * n * case["width"] + 7 * 4 * n + rows * (4 + 4 + 8 + (4 + 8 * words)), "flops": 0}
     if case["op"] == "append":
         return {"bytes": 2 * case["rows"] * (case["heads"] * case["dim"] * (SIZE[case["src"]] + SIZE[case["dst"]]) + 4),
                 "flops": 0}
@@ -270,7 +270,7 @@ def _plan_plain(s):
     slot = torch.where(ok[req], page * ps + token % ps, -1)
     out = {"table": table_out, "held": (held + torch.where(ok, need, 0)).int(), "count": (s["count"] - taken).int(),
            "row_start": row_start.int(), "row_req": req.int(), "slot": slot,
-           "status": (~ok.all()).int().reshape(1)}
+           "status": (~ok).int()}
     if s["parents"] is None:
         out["pos"] = token.int()
     else:
@@ -364,7 +364,7 @@ def _plan_own(s):
            "count": torch.empty_like(s["count"]), "row_start": torch.empty(n + 1, dtype=torch.int32, device=dev),
            "row_req": torch.empty(s["rows"], dtype=torch.int32, device=dev),
            "slot": torch.empty(s["rows"], dtype=torch.int64, device=dev),
-           "status": torch.empty(1, dtype=torch.int32, device=dev),
+           "status": torch.empty(n, dtype=torch.int32, device=dev),
            "pos": torch.empty(s["rows"], dtype=torch.int32, device=dev)}
     if s["parents"] is not None:
         out["mask"] = torch.empty(s["rows"], s["words"], dtype=torch.int64, device=dev)
