@@ -133,6 +133,38 @@ class ExecRecord(C.Structure):
                 ("device_ms", C.c_double), ("family", C.c_int32 * 6), ("precision_source", C.c_char * 32)]
 
 
+# element types of the serving operators (fwhip.h FWHIP_T_*)
+T_F32, T_F16, T_BF16 = range(3)
+
+
+class PagedPlanArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_req", "width", "page_size", "n_rows", "n_free", "mask_words")] + [
+        (n, C.c_void_p) for n in ("len", "n_new", "parents", "table", "held", "free_pages", "free_count", "table_out",
+                                  "held_out", "count_out", "row_start", "row_req", "pos", "slot", "mask", "status")]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("src_dtype", "cache_dtype", "n_rows", "n_heads", "head_dim", "n_pages",
+                                         "page_size")] + [
+        (n, C.c_int64) for n in ("k_row", "k_head", "v_row", "v_head", "page_stride", "token_stride", "head_stride")] + [
+        (n, C.c_void_p) for n in ("k", "v", "slot", "k_cache", "v_cache")]
+
+
+class TreeAttnArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "n_req", "n_rows", "n_heads", "n_kv_heads", "head_dim", "n_pages",
+                                         "page_size", "width", "max_new", "max_len", "mask_words")] + [
+        ("scale", C.c_float)] + [
+        (n, C.c_int64) for n in ("table_stride", "q_row", "q_head", "out_row", "out_head", "page_stride",
+                                 "token_stride", "head_stride")] + [
+        (n, C.c_void_p) for n in ("q", "k_cache", "v_cache", "table", "len", "row_start", "mask", "out", "workspace")] + [
+        ("workspace_bytes", C.c_uint64)]
+
+
+class Q4LinearArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "scale_dtype", "group", "m", "n", "k")] + [
+        ("ldx", C.c_int64), ("ldy", C.c_int64)] + [(n, C.c_void_p) for n in ("x", "q", "scale", "minimum", "bias", "y")]
+
+
 def ptr(arr, ctype):
     """Pointer to a contiguous numpy array's buffer (caller keeps `arr` alive)."""
     if arr is None:

@@ -27,6 +27,7 @@ struct fwhip_ctx {
     int device = 0;
     int n_cu = 0;
     hipStream_t stream = nullptr;
+    bool own_stream = true; // false: the caller's (fwhip_init_on_stream)
     std::atomic<int> cancel{0};
     bool timing = false;
     std::vector<fw_event_pair> pending;

@@ -37,7 +37,7 @@ extern "C" int32_t fwhip_abi_version(void) { return FWHIP_ABI_VERSION; }
 
 // ---------------------------------------------------------------------------
 // context
-extern "C" fwhip_status fwhip_init(int32_t device, fwhip_ctx **out) {
+static fwhip_status ctx_new(int32_t device, bool own_stream, hipStream_t stream, fwhip_ctx **out) {
     if (!out) return fw_fail(FWHIP_ERR_INVALID, "fwhip_init: out is NULL");
     *out = nullptr;
     int n = 0;
@@ -53,7 +53,9 @@ extern "C" fwhip_status fwhip_init(int32_t device, fwhip_ctx **out) {
     fwhip_ctx *c = new fwhip_ctx();
     c->device = device;
     c->n_cu = prop.multiProcessorCount;
-    if (hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking) != hipSuccess) {
+    c->own_stream = own_stream;
+    c->stream = stream;
+    if (own_stream && hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking) != hipSuccess) {
         delete c;
         return fw_fail(FWHIP_ERR_GENERIC, "hipStreamCreate failed");
     }
@@ -87,6 +89,11 @@ extern "C" fwhip_status fwhip_init(int32_t device, fwhip_ctx **out) {
     return FWHIP_OK;
 }
 
+extern "C" fwhip_status fwhip_init(int32_t device, fwhip_ctx **out) { return ctx_new(device, true, nullptr, out); }
+extern "C" fwhip_status fwhip_init_on_stream(int32_t device, void *stream, fwhip_ctx **out) {
+    return ctx_new(device, false, (hipStream_t)stream, out);
+}
+
 void fw_ovf_clear(fwhip_ctx *c) { fw_launch_fill_u16(c->stream, (uint16_t *)c->ovf_dev, 2, 0); }
 void fw_ovf_fetch(fwhip_ctx *c) {
     (void)hipMemcpyAsync(c->ovf_host, c->ovf_dev, sizeof(int), hipMemcpyDeviceToHost, c->stream);
@@ -113,7 +120,7 @@ extern "C" void fwhip_destroy(fwhip_ctx *c) {
     if (c->am_scratch) hipFree(c->am_scratch);
     if (c->ovf_dev) hipFree(c->ovf_dev);
     if (c->ovf_host) hipHostFree(c->ovf_host);
-    hipStreamDestroy(c->stream);
+    if (c->own_stream) hipStreamDestroy(c->stream);
     delete c;
 }
 
@@ -1226,7 +1233,10 @@ static bool capture_step_impl(fwhip_dstate *st, const fwhip_filter *filt) {
         st->graph = nullptr;
     }
     hipStream_t s = st->dec->ctx->stream;
-    if (hipStreamBeginCapture(s, hipStreamCaptureModeThreadLocal) != hipSuccess) return false;
+    if (hipStreamBeginCapture(s, hipStreamCaptureModeThreadLocal) != hipSuccess) {
+        (void)hipGetLastError(); // the default stream (fwhip_init_on_stream) takes no capture
+        return false;
+    }
     greedy_step(st, filt, false);
     hipGraph_t g = nullptr;
     if (hipStreamEndCapture(s, &g) != hipSuccess || !g) {
@@ -1438,7 +1448,10 @@ static bool win_capture(fwhip_dstate *st, const FwWinCfg &cfg) {
         st->wgraph = nullptr;
     }
     hipStream_t s = st->dec->ctx->stream;
-    if (hipStreamBeginCapture(s, hipStreamCaptureModeThreadLocal) != hipSuccess) return false;
+    if (hipStreamBeginCapture(s, hipStreamCaptureModeThreadLocal) != hipSuccess) {
+        (void)hipGetLastError(); // the default stream (fwhip_init_on_stream) takes no capture
+        return false;
+    }
     win_step(st, cfg);
     hipGraph_t g = nullptr;
     if (hipStreamEndCapture(s, &g) != hipSuccess || !g) {

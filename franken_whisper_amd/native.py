@@ -25,6 +25,7 @@ _i64p = C.POINTER(C.c_int64)
 # name -> (restype, argtypes); every symbol include/fwhip.h declares
 SIGNATURES = {
     "fwhip_init": (C.c_int32, [C.c_int32, C.POINTER(_vp)]),
+    "fwhip_init_on_stream": (C.c_int32, [C.c_int32, _vp, C.POINTER(_vp)]),
     "fwhip_destroy": (None, [_vp]),
     "fwhip_last_error": (C.c_char_p, []),
     "fwhip_abi_version": (C.c_int32, []),
@@ -95,6 +96,12 @@ SIGNATURES = {
     "fwhip_dequant": (C.c_int32, [_vp, C.c_int32, _vp, C.c_uint64, C.c_int64, _vp]),
     "fwhip_encoder_load_ggml": (C.c_int32, [_vp, _vp, C.c_int32, C.POINTER(_vp)]),
     "fwhip_decoder_load_ggml": (C.c_int32, [_vp, _vp, C.c_int32, C.POINTER(_vp)]),
+    "fwhip_paged_plan": (C.c_int32, [_vp, C.POINTER(abi.PagedPlanArgs)]),
+    "fwhip_paged_append": (C.c_int32, [_vp, C.POINTER(abi.PagedAppendArgs)]),
+    "fwhip_tree_attn": (C.c_int32, [_vp, C.POINTER(abi.TreeAttnArgs)]),
+    "fwhip_tree_attn_workspace": (C.c_int32, [C.c_int32] * 6 + [C.POINTER(C.c_uint64)]),
+    "fwhip_q4_linear": (C.c_int32, [_vp, C.POINTER(abi.Q4LinearArgs)]),
+    "fwhip_q4_planes": (C.c_int32, [_vp, C.c_int32, _vp, C.c_uint64, C.c_int32, C.c_int32, _vp, _vp, _vp]),
 }
 
 _lib = None
@@ -159,9 +166,15 @@ def mel_frames(n_samples: int) -> int:
 
 
 class Context:
-    def __init__(self, device: int = 0):
+    def __init__(self, device: int = 0, stream: int | None = None):
+        """stream: the handle (hipStream_t as an integer, 0 for the default
+        stream) of a stream of the caller's to queue all work on; None: a
+        stream of the context's own."""
         h = _vp()
-        check(lib().fwhip_init(device, C.byref(h)))
+        if stream is None:
+            check(lib().fwhip_init(device, C.byref(h)))
+        else:
+            check(lib().fwhip_init_on_stream(device, stream, C.byref(h)))
         self.h = h
 
     def array(self, a: np.ndarray) -> DeviceArray:

@@ -186,6 +186,13 @@ typedef struct fwhip_exec_record {
 /* Open device `device` and create a context with its own stream.
  * FWHIP_ERR_UNSUPPORTED when no gfx950 device is visible. */
 fwhip_status fwhip_init(int32_t device, fwhip_ctx **out);
+/* The same on a stream of the caller's: `stream` is a hipStream_t of `device`
+ * (NULL: the device's default stream), and every call on the context queues its
+ * work there, so it is ordered with whatever else the caller queues on it.  The
+ * stream stays the caller's: it must outlive the context, which never destroys
+ * it.  No counterpart in the reference: for hosts that own their streams, such
+ * as a torch program or one that captures its step into a HIP graph. */
+fwhip_status fwhip_init_on_stream(int32_t device, void *stream, fwhip_ctx **out);
 void fwhip_destroy(fwhip_ctx *ctx);
 const char *fwhip_last_error(void);
 int32_t fwhip_abi_version(void);
@@ -663,6 +670,165 @@ fwhip_status fwhip_encoder_load_ggml(fwhip_ctx *ctx, const fwhip_ggml *g, int32_
  * decoder.rs:599-720), so every linear and the token embedding must be stored
  * as f16 (else FWHIP_ERR_UNSUPPORTED "cpu:ggml-<type>-linear: ..."). */
 fwhip_status fwhip_decoder_load_ggml(fwhip_ctx *ctx, const fwhip_ggml *g, int32_t arm, fwhip_decoder **out);
+
+/* ---- decoding with drafted tokens ----------------------------------------- */
+
+/* The operators of a decode step that verifies drafted tokens for a batch of
+ * requests over a paged K/V cache, and the linears of a 4-bit model.  The
+ * reference decodes one token per stream over a contiguous cache (KvCache,
+ * nn.rs:5138) and has no counterpart; they stand beside fwhip_dequant and
+ * fwhip_layer_norm as operators on device memory.
+ *
+ * A step: fwhip_paged_plan gives the requests' pages, slots, positions and
+ * ancestor masks from their lengths; the projections (fwhip_q4_linear) make
+ * q/k/v rows; fwhip_paged_append stores K and V; fwhip_tree_attn attends.
+ *
+ * All four only queue work on the context's stream: they allocate nothing,
+ * wait for nothing and copy nothing to the host, so a step can be captured
+ * into a HIP graph.  Pointers are device addresses.  What the host can see is
+ * checked before anything is queued (FWHIP_ERR_INVALID, or
+ * FWHIP_ERR_UNSUPPORTED for a form that is not built); what only the device
+ * knows (lengths, page numbers, slots) is checked by the kernels, which never
+ * read or write outside the arrays described here.  Outputs must not overlap
+ * inputs except where said. */
+
+/* Element types of these operators' tensors. */
+#define FWHIP_T_F32 0
+#define FWHIP_T_F16 1
+#define FWHIP_T_BF16 2
+
+/* fwhip_paged_plan: from the lengths of n_req requests, where the step's new
+ * tokens go.  Request r holds held[r] pages (the first entries of its table
+ * row) for len[r] cached tokens and brings n_new[r] new ones, which take the
+ * token positions len[r] + 0 .. n_new[r] - 1 of the cache.
+ *   pages     request r needs ceil((len + n_new) / page_size) - held more pages
+ *             when that is positive.  Requests take them in order from the top
+ *             of the free list (free_pages[count - 1] first) for as long as the
+ *             running sum of needs stays within count; one that does not fit,
+ *             or whose table row has no room, gets none (status 1), and so do
+ *             all later ones that need pages.
+ *   rows      the new tokens of all requests in order: row_start [n_req + 1],
+ *             and per row row_req (its request), slot (page * page_size +
+ *             offset, -1 when its request got no pages) and pos.
+ *   tree      with parents (per row the index of its parent within the
+ *             request's new tokens, smaller than its own, or -1 for a child of
+ *             the cached text) mask receives each row's ancestors, itself among
+ *             them, as bits of mask_words 64-bit words (bit i: the request's
+ *             new token i), and pos is len + the number of ancestors above it.
+ *             A request has at most 64 * mask_words new tokens then, and
+ *             mask_words <= 4.  Without parents the new tokens are a chain:
+ *             pos = len + i, and mask is NULL.
+ *   status    [n_req]: 0, or bits 1 no pages, 2 a negative or overlong length
+ *             (len, n_new or held; rows past n_rows are cut), 4 a parent out of
+ *             order (taken as -1) or too many new tokens for the mask (empty
+ *             masks).
+ * table_out is table with the new entries, held_out and count_out what remains
+ * of it; table_out may be table itself (then only new entries are written). */
+typedef struct fwhip_paged_plan_args {
+    int32_t n_req, width, page_size;   /* requests; table columns; tokens per page */
+    int32_t n_rows, n_free;            /* capacity of the row arrays; entries of free_pages */
+    int32_t mask_words;                /* 64-bit words per mask row (0 without parents) */
+    const int32_t *len, *n_new;        /* [n_req] */
+    const int32_t *parents;            /* [n_rows] or NULL */
+    const int32_t *table;              /* [n_req, width] */
+    const int32_t *held;               /* [n_req] */
+    const int32_t *free_pages, *free_count; /* [n_free]; [1]: how many of them are free */
+    int32_t *table_out, *held_out, *count_out; /* [n_req, width], [n_req], [1] */
+    int32_t *row_start, *row_req, *pos; /* [n_req + 1], [n_rows], [n_rows] */
+    int64_t *slot;                     /* [n_rows] */
+    uint64_t *mask;                    /* [n_rows, mask_words] or NULL */
+    int32_t *status;                   /* [n_req] */
+} fwhip_paged_plan_args;
+fwhip_status fwhip_paged_plan(fwhip_ctx *ctx, const fwhip_paged_plan_args *args);
+
+/* fwhip_paged_append: rows of K and V into the cache, each value rounded to the
+ * cache's type (to nearest, ties to even).  Row i goes to slot[i] = page *
+ * page_size + offset; a slot outside [0, n_pages * page_size) is skipped.
+ * Slots are different from each other: of two rows with one slot either may
+ * stay.  Strides are in elements; head_dim elements lie next to each other. */
+typedef struct fwhip_paged_append_args {
+    int32_t src_dtype, cache_dtype;    /* FWHIP_T_* */
+    int32_t n_rows, n_heads, head_dim; /* K/V heads */
+    int32_t n_pages, page_size;
+    int64_t k_row, k_head, v_row, v_head;           /* strides of k and v */
+    int64_t page_stride, token_stride, head_stride; /* strides of both caches */
+    const void *k, *v;
+    const int64_t *slot;
+    void *k_cache, *v_cache;
+} fwhip_paged_append_args;
+fwhip_status fwhip_paged_append(fwhip_ctx *ctx, const fwhip_paged_append_args *args);
+
+/* fwhip_tree_attn: out_i = sum_j p_ij v_j, p_i = softmax_j(scale * q_i . k_j)
+ * over the keys that row i sees: all len[r] cached tokens of its request r, and
+ * of the request's new tokens (cached behind them at len[r] + t) those whose
+ * bit is set in mask row i, or t <= its own index where mask is NULL (a causal
+ * chain: prompts, single tokens).  A row that sees no key is zero.  What a row
+ * does not see never reaches it, whatever it holds (infinities and NaN too).
+ * Request r has rows row_start[r] .. row_start[r + 1] - 1 of q and out; rows
+ * outside [row_start[0], row_start[n_req]) are neither read nor written.
+ * Query head h reads K/V head h / (n_heads / n_kv_heads).
+ * max_new and max_len bound a request's new tokens and its len + new tokens
+ * (the host's view of the step: larger ones only cost time).  Rows of a request
+ * that exceeds a bound, has a negative length, or sees a token whose table entry
+ * is no page of [0, n_pages) come out as NaN; such entries are never followed.
+ * q, the caches and out share one type; scores, softmax and sums are f32.
+ * head_dim is 64 or 128; addresses and strides are multiples of 16 bytes, the
+ * strides non-negative.  workspace (16-byte aligned) holds the partial results
+ * of a long cache that is split over workgroups: at least
+ * fwhip_tree_attn_workspace bytes for the same sizes, and for the call alone
+ * until it has run (two graphs that may replay at once need one each). */
+typedef struct fwhip_tree_attn_args {
+    int32_t dtype;                     /* FWHIP_T_* */
+    int32_t n_req, n_rows;             /* requests; rows of q and out */
+    int32_t n_heads, n_kv_heads, head_dim;
+    int32_t n_pages, page_size, width; /* the cache; table columns */
+    int32_t max_new, max_len;
+    int32_t mask_words;                /* 64-bit words per mask row, 64 * mask_words >= max_new (0 without mask) */
+    float scale;
+    int64_t table_stride;              /* elements between table rows */
+    int64_t q_row, q_head, out_row, out_head;       /* strides, elements */
+    int64_t page_stride, token_stride, head_stride; /* of both caches */
+    const void *q, *k_cache, *v_cache;
+    const int32_t *table, *len, *row_start; /* [n_req, width], [n_req], [n_req + 1] */
+    const uint64_t *mask;              /* [n_rows, mask_words] or NULL */
+    void *out;
+    void *workspace;
+    uint64_t workspace_bytes;
+} fwhip_tree_attn_args;
+fwhip_status fwhip_tree_attn(fwhip_ctx *ctx, const fwhip_tree_attn_args *args);
+/* Workspace bytes of a call of these sizes (0: none needed); grows with each
+ * of n_req, max_new and max_len, so one of the largest step serves all. */
+fwhip_status fwhip_tree_attn_workspace(int32_t n_req, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                       int32_t max_new, int32_t max_len, uint64_t *bytes);
+
+/* fwhip_q4_linear: y = x W^T (+ bias) for m rows of x and 4-bit weights W [n, k]
+ * in planes: q [n, k / 2] bytes, where byte j of each 16 holds weight j of its
+ * 32 in the low and weight j + 16 in the high half (ggml's order), and a scale,
+ * optionally a minimum, for every `group` weights of a row ([n, k / group]):
+ *   w = (code - 8) * scale, or code * scale + minimum.
+ * x and y share a type.  Codes are multiplied as whole numbers, summed per group
+ * in f32 and scaled in f32; y is rounded once.
+ * group is 32, 64 or 128 and divides k; q 16-byte aligned, ldx >= k, ldy >= n. */
+typedef struct fwhip_q4_linear_args {
+    int32_t dtype, scale_dtype;        /* of x and y: FWHIP_T_*; of the planes: FWHIP_T_F16 or FWHIP_T_F32 */
+    int32_t group, m, n, k;
+    int64_t ldx, ldy;                  /* elements between rows */
+    const void *x;
+    const uint8_t *q;
+    const void *scale, *minimum;       /* minimum: NULL for code - 8 */
+    const float *bias;                 /* [n] or NULL */
+    void *y;
+} fwhip_q4_linear_args;
+fwhip_status fwhip_q4_linear(fwhip_ctx *ctx, const fwhip_q4_linear_args *args);
+
+/* A ggml payload (fwhip_ggml_tensor_raw, on the device) of a [rows, k] linear as
+ * the planes of fwhip_q4_linear with group 32: FWHIP_GGML_Q4_0 (f16 scales, no
+ * minimum), FWHIP_GGML_Q4_1 (f16 scales and minimums) and FWHIP_GGML_Q4_K (f32
+ * scales and minimums, the products of dequant_q4_k, ggml.rs:117-157).  raw 4-byte,
+ * the planes 16-byte aligned; raw_bytes must be the payload's length.  Queued on
+ * the context's stream. */
+fwhip_status fwhip_q4_planes(fwhip_ctx *ctx, int32_t ggml_dtype, const void *raw, uint64_t raw_bytes, int32_t rows,
+                             int32_t k, uint8_t *q, void *scale, void *minimum);
 
 #ifdef __cplusplus
 }
