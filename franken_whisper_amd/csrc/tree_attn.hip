@@ -6,6 +6,7 @@
 // over the keys with a running maximum m and sum l:
 //   m' = max(m, max_j z_j),  l' = l e^(m-m') + sum_j e^(z_j-m'),  o' likewise.
 #include <algorithm>
+#include <type_traits>
 
 #include "fw_device.h"
 #include "fw_paged.h"
@@ -20,88 +21,556 @@ struct TreeP {
     const int32_t *table, *len, *row_start;
     const uint64_t *mask;
     void *out;
+    // how the call is cut (tree_cut): key splits and their length, row tiles and
+    // their rows, the parts [request, tile, K/V head, split, row, D + 4]
+    int splits, chunk, tiles, tile_rows;
+    float *parts;
 };
 
-// One wave per (row, head): a lane per key for the scores, a lane per output
-// feature (D / 64 of them) for the sum.
-template <typename T, int D>
-__global__ void __launch_bounds__(64) k_tree_attn(TreeP p) {
-    __shared__ float sq[D], sp[64];
-    __shared__ int64_t sat[64];
-    const int lane = threadIdx.x, h = blockIdx.y, i = blockIdx.x;
-    const int r = blockIdx.z, kvh = h / (p.heads / p.kv_heads);
-    const int row0 = min(max(p.row_start[r], 0), p.n_rows), row1 = min(p.row_start[r + 1], p.n_rows);
-    const int n = row1 - row0, len = p.len[r];
-    // rows of this request past max_new are marked too
-    for (int row = row0 + i; row < row1; row += gridDim.x) {
-        T *out = (T *)p.out + (int64_t)row * p.out_row + (int64_t)h * p.out_head;
-        if (len < 0 || n > p.max_new || (int64_t)len + n > p.max_len) {
-            for (int e = lane; e < D; e += 64) out[e] = fw_cvt<T>(__builtin_nanf(""));
-            continue;
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+// Products of 16 x 16 tiles.  A lane l holds row (A) or column (B) l % 16 of an
+// operand and its quarter c = l / 16 of the inner dimension; of the result,
+// column l % 16 and rows 4 c + 0..3.  Both inner dimensions may be permuted as
+// long as the operands agree, which is what lets scores (keys x rows) become
+// weights (keys x rows) of the second product without leaving their lanes.
+template <typename T>
+struct Mma;
+template <>
+struct Mma<fw_f16> {
+    static constexpr int KT = 2; // key tiles a step: one product of inner dimension 32 takes 32 keys
+    static __device__ __forceinline__ f4 dot(u4 a, u4 b, f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    }
+    // p = hi + lo up to 2^-20 of p: two f16 of 11 bits each, cut
+    static __device__ __forceinline__ void split(const float *p, u4 &hi, u4 &lo) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const auto h = __builtin_amdgcn_cvt_pkrtz(p[2 * i], p[2 * i + 1]);
+            const auto l = __builtin_amdgcn_cvt_pkrtz(p[2 * i] - (float)h[0], p[2 * i + 1] - (float)h[1]);
+            hi[i] = __builtin_bit_cast(uint32_t, h);
+            lo[i] = __builtin_bit_cast(uint32_t, l);
         }
-        const int me = row - row0;
-        __syncthreads();
-        for (int e = lane; e < D; e += 64)
-            sq[e] = fw_to_f32(((const T *)p.q)[(int64_t)row * p.q_row + (int64_t)h * p.q_head + e]);
-        float m = -INFINITY, l = 0.0f, o[D / 64] = {};
-        bool any = false;
-        __syncthreads();
-        for (int j0 = 0; j0 < len + n; j0 += 64) {
-            const int j = j0 + lane;
-            bool sees = j < len + n;
-            if (sees && j >= len) {
-                const int t = j - len;
-                sees = p.mask ? (p.mask[(int64_t)row * p.words + (t >> 6)] >> (t & 63)) & 1 : t <= me;
+    }
+};
+template <>
+struct Mma<fw_bf16> {
+    static constexpr int KT = 2;
+    static __device__ __forceinline__ f4 dot(u4 a, u4 b, f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    }
+    // p = hi + lo up to 2^-16 of p: the upper half of the f32, and the rest rounded to 8 bits
+    static __device__ __forceinline__ void split(const float *p, u4 &hi, u4 &lo) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t x = __float_as_uint(p[2 * i]), y = __float_as_uint(p[2 * i + 1]);
+            hi[i] = __builtin_amdgcn_perm(y, x, 0x07060302);
+            const b2 l = {(__bf16)(p[2 * i] - __uint_as_float(x & 0xffff0000u)),
+                          (__bf16)(p[2 * i + 1] - __uint_as_float(y & 0xffff0000u))};
+            lo[i] = __builtin_bit_cast(uint32_t, l);
+        }
+    }
+};
+template <>
+struct Mma<float> {
+    static constexpr int KT = 1;
+    static __device__ __forceinline__ f4 dot(u4 a, u4 b, f4 c) {
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[t]), __uint_as_float(b[t]), c, 0, 0, 0);
+        return c;
+    }
+};
+
+// Over the four lanes that share l % 16.
+__device__ __forceinline__ float quarters_max(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float quarters_sum(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Weights are 2^15 e^(z - m): the factor cancels in o / l and keeps f16 weights
+// of far smaller keys (down to 2^-29 of the largest) in the normal range.
+#define TREE_BIAS 15.0f
+__device__ __forceinline__ float tree_base(float m) { return m == -INFINITY ? 0.0f : m - TREE_BIAS; }
+
+template <typename T>
+__device__ __forceinline__ bool has_nonfinite(u4 v) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) bad |= (v[i] & 0x7f800000u) == 0x7f800000u;
+        else {
+            constexpr uint32_t E = std::is_same<T, fw_f16>::value ? 0x7c00u : 0x7f80u;
+            bad |= (v[i] & E) == E || (v[i] >> 16 & E) == E;
+        }
+    }
+    return bad;
+}
+template <typename T>
+__device__ __forceinline__ u4 drop_nonfinite(u4 v) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) v[i] = (v[i] & 0x7f800000u) == 0x7f800000u ? 0 : v[i];
+        else {
+            constexpr uint32_t E = std::is_same<T, fw_f16>::value ? 0x7c00u : 0x7f80u;
+            if ((v[i] & E) == E) v[i] &= 0xffff0000u;
+            if ((v[i] >> 16 & E) == E) v[i] &= 0xffffu;
+        }
+    }
+    return v;
+}
+
+// What a block finds about its request; bad: out of the call's bounds.
+struct TreeReq {
+    int row0, n, len;
+    bool bad;
+};
+__device__ __forceinline__ TreeReq tree_req(const TreeP &p, int r) {
+    TreeReq q;
+    q.row0 = min(max(p.row_start[r], 0), p.n_rows);
+    q.n = max(min(p.row_start[r + 1], p.n_rows) - q.row0, 0);
+    q.len = p.len[r];
+    q.bad = q.len < 0 || q.n > p.max_new || (int64_t)q.len + q.n > p.max_len;
+    return q;
+}
+// Whether new token i of a request with n of them sees any key.
+__device__ __forceinline__ bool tree_sees_any(const TreeP &p, const TreeReq &q, int i) {
+    if (q.len > 0 || !p.words) return true;
+    uint64_t any = 0;
+    for (int w = 0; w * 64 < q.n; w++) {
+        const uint64_t m = p.mask[(int64_t)(q.row0 + i) * p.words + w];
+        any |= q.n - w * 64 >= 64 ? m : m & ((1ull << (q.n - w * 64)) - 1);
+    }
+    return any != 0;
+}
+
+template <typename T>
+struct Vec4 {
+    typedef uint2 type;
+};
+template <>
+struct Vec4<float> {
+    typedef float4 type;
+};
+template <typename T>
+__device__ __forceinline__ typename Vec4<T>::type pack4(f4 v) {
+    if constexpr (sizeof(T) == 4) return make_float4(v[0], v[1], v[2], v[3]);
+    else
+        return make_uint2(fw_cvt<T>(v[0]).b | (uint32_t)fw_cvt<T>(v[1]).b << 16,
+                          fw_cvt<T>(v[2]).b | (uint32_t)fw_cvt<T>(v[3]).b << 16);
+}
+
+// A block: one K/V head of one request, RT * 16 of its query rows (new token x
+// query head of the group), and one chunk of its keys.  Its four waves take the
+// chunk's steps of KT * 16 keys in turn, each with a running maximum, sum and
+// output of its own for all rows, so K and V are read once a block; they are
+// joined through LDS at the end.  A wave's K tile goes from memory to the lanes
+// that multiply it; its V tile passes through LDS, where the transposing read
+// gives each lane the keys of one feature.  The next step's tiles are in flight
+// while a step computes.
+template <typename T, int D, int RT>
+__global__ void __launch_bounds__(256, RT == 4 ? 1 : 2) k_tree_attn(TreeP p) {
+    constexpr int KT = Mma<T>::KT, KEYS = 16 * KT, NS = D * (int)sizeof(T) / 64, DT = D / 16;
+    constexpr int VROW = D * (int)sizeof(T) + 32; // bytes of a V row in LDS: rows 8 banks apart
+    constexpr int VBYTES = 4 * KEYS * VROW, OBYTES = RT * 16 * D * 4;
+    __shared__ __attribute__((aligned(16))) char lds[VBYTES > OBYTES ? VBYTES : OBYTES];
+    __shared__ float sm[4][RT * 16], sl[4][RT * 16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4;
+    const int group = p.heads / p.kv_heads;
+    const int split = blockIdx.x, kvh = blockIdx.y % p.kv_heads, tile = blockIdx.y / p.kv_heads, r = blockIdx.z;
+    const TreeReq rq = tree_req(p, r);
+    const bool whole = p.splits == 1;
+    if (rq.bad) { // may have more rows than there are tiles
+        if (whole && tile == 0)
+            for (int64_t e = threadIdx.x; e < (int64_t)rq.n * group * D; e += 256) {
+                const int64_t i = e / D / group, h = kvh * group + e / D % group;
+                ((T *)p.out)[(rq.row0 + i) * p.out_row + h * p.out_head + e % D] = fw_cvt<T>(__builtin_nanf(""));
             }
-            float z = -INFINITY;
-            int64_t at = 0;
-            if (sees) {
-                const uint32_t pi = fw_div((uint32_t)j, p.page);
-                const int id = p.table[(int64_t)r * p.table_stride + pi];
-                if (id < 0 || id >= p.n_pages) {
-                    z = __builtin_nanf("");
-                    at = -1;
+        return;
+    }
+    const int total = rq.n * group, t0 = tile * RT * 16;
+    if (t0 >= total) return;
+    const int end = rq.len + rq.n; // keys of the request
+    // a chain's rows see no further than the tile's last token
+    const int tile_end = p.words ? end : min(end, rq.len + (min(t0 + RT * 16, total) - 1) / group + 1);
+    const int first = split * p.chunk, last = min(tile_end, first + p.chunk);
+    if (!whole && first >= tile_end) return; // the join reads no part of it
+
+    // query rows
+    int node[RT];
+    int64_t qat[RT];
+    u4 q[RT][NS];
+#pragma unroll
+    for (int x = 0; x < RT; x++) {
+        const int t = min(t0 + x * 16 + lr, total - 1);
+        node[x] = t / group;
+        qat[x] = (int64_t)(kvh * group + t % group);
+        const T *at = (const T *)p.q + (int64_t)(rq.row0 + node[x]) * p.q_row + qat[x] * p.q_head;
+#pragma unroll
+        for (int s = 0; s < NS; s++) q[x][s] = *(const u4 *)((const char *)at + s * 64 + c * 16);
+    }
+    const float zs = p.scale * 1.44269504088896340736f; // scores in base 2
+    char *vt = lds + wave * KEYS * VROW;
+    const int32_t *trow = p.table + (int64_t)r * p.table_stride;
+
+    f4 o[RT][DT];
+    float m[RT], l[RT];
+    for (int careful = 0; careful < 2; careful++) {
+#pragma unroll
+        for (int x = 0; x < RT; x++) {
+            m[x] = -INFINITY;
+            l[x] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[x][d] = f4{};
+        }
+        int j0 = first + wave * KEYS;
+        int pid[KT];        // the next step's pages
+        int64_t off[KT];    // this step's keys, -1 where there is none
+        u4 kf[KT][NS], vf[KT][NS];
+        auto pages = [&](int j) {
+#pragma unroll
+            for (int k = 0; k < KT; k++) {
+                const int key = j + k * 16 + lr;
+                pid[k] = key < last ? trow[fw_div((uint32_t)key, p.page)] : -1;
+            }
+        };
+        auto offsets = [&](int j) {
+#pragma unroll
+            for (int k = 0; k < KT; k++) {
+                const uint32_t key = (uint32_t)(j + k * 16 + lr), pi = fw_div(key, p.page);
+                off[k] = (uint32_t)pid[k] < (uint32_t)p.n_pages
+                             ? (int64_t)pid[k] * p.page_stride + (int64_t)(key - pi * p.page.d) * p.token_stride +
+                                   (int64_t)kvh * p.head_stride
+                             : -1;
+            }
+        };
+        auto load = [&](const void *base, u4 (*f)[NS]) {
+#pragma unroll
+            for (int k = 0; k < KT; k++) {
+                const char *at = (const char *)((const T *)base + max(off[k], (int64_t)0)) + c * 16;
+#pragma unroll
+                for (int s = 0; s < NS; s++) f[k][s] = *(const u4 *)(at + s * 64);
+            }
+        };
+        if (j0 < last) {
+            pages(j0);
+            offsets(j0);
+            load(p.kc, kf);
+            load(p.vc, vf);
+            pages(j0 + 4 * KEYS);
+        }
+        for (; j0 < last; j0 += 4 * KEYS) {
+            int64_t here[KT];
+#pragma unroll
+            for (int k = 0; k < KT; k++) here[k] = off[k];
+            // scores of this step: keys 16 k + 4 c + 0..3 of row lr
+            f4 z[RT][KT];
+#pragma unroll
+            for (int x = 0; x < RT; x++)
+#pragma unroll
+                for (int k = 0; k < KT; k++) {
+                    f4 a = {};
+#pragma unroll
+                    for (int s = 0; s < NS; s++) a = Mma<T>::dot(kf[k][s], q[x][s], a);
+                    z[x][k] = a * zs;
+                }
+            const bool edge = j0 + KEYS > min(rq.len, last); // new tokens, or the chunk's end
+            const bool lost = __any(here[0] < 0 || here[KT - 1] < 0); // beyond the end, or no page
+            if (lost) {
+#pragma unroll
+                for (int k = 0; k < KT; k++)
+                    if (here[k] < 0)
+#pragma unroll
+                        for (int s = 0; s < NS; s++) vf[k][s] = u4{};
+            }
+            if (careful) {
+#pragma unroll
+                for (int k = 0; k < KT; k++)
+#pragma unroll
+                    for (int s = 0; s < NS; s++) vf[k][s] = drop_nonfinite<T>(vf[k][s]);
+            }
+            wave_fence();
+#pragma unroll
+            for (int k = 0; k < KT; k++)
+#pragma unroll
+                for (int s = 0; s < NS; s++) *(u4 *)(vt + (k * 16 + lr) * VROW + s * 64 + c * 16) = vf[k][s];
+            wave_fence();
+            if (j0 + 4 * KEYS < last) {
+                offsets(j0 + 4 * KEYS);
+                load(p.kc, kf);
+                load(p.vc, vf);
+                pages(j0 + 8 * KEYS);
+            }
+            uint32_t sees[RT];
+#pragma unroll
+            for (int x = 0; x < RT; x++) sees[x] = 0xffffffffu;
+            if (edge || lost) {
+#pragma unroll
+                for (int x = 0; x < RT; x++) {
+                    sees[x] = 0;
+#pragma unroll
+                    for (int k = 0; k < KT; k++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int key = j0 + k * 16 + 4 * c + i, t = key - rq.len;
+                            bool yes = key < last;
+                            if (yes && t >= 0)
+                                yes = p.words ? p.mask[(int64_t)(rq.row0 + node[x]) * p.words + (t >> 6)] >> (t & 63) & 1
+                                              : t <= node[x];
+                            // a key whose table entry is no page makes its rows NaN
+                            const int64_t there = __shfl(here[k], 4 * c + i);
+                            z[x][k][i] = !yes ? -INFINITY : there < 0 ? __builtin_nanf("") : z[x][k][i];
+                            sees[x] |= (uint32_t)yes << (4 * k + i);
+                        }
+                }
+            }
+            // weights
+            u4 hi[RT], lo[RT];
+            float pw[RT][4 * KT];
+#pragma unroll
+            for (int x = 0; x < RT; x++) {
+                float mx = z[x][0][0];
+#pragma unroll
+                for (int k = 0; k < KT; k++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) mx = fmaxf(mx, z[x][k][i]);
+                mx = quarters_max(mx);
+                if (__any(mx > m[x])) {
+                    const float mn = fmaxf(mx, m[x]), f = __builtin_amdgcn_exp2f(m[x] - TREE_BIAS - tree_base(mn));
+                    m[x] = mn;
+                    l[x] *= f;
+#pragma unroll
+                    for (int d = 0; d < DT; d++) o[x][d] *= f;
+                }
+                const float base = tree_base(m[x]);
+#pragma unroll
+                for (int k = 0; k < KT; k++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        pw[x][4 * k + i] = __builtin_amdgcn_exp2f(z[x][k][i] - base);
+                        l[x] += pw[x][4 * k + i];
+                    }
+                if constexpr (sizeof(T) == 2) Mma<T>::split(pw[x], hi[x], lo[x]);
+            }
+            // outputs: features 16 d + 4 c + 0..3 of row lr
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                if constexpr (sizeof(T) == 2) {
+                    u4 v;
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const char *at = vt + (k * 16 + 4 * c + (lr >> 2)) * VROW + d * 32 + (lr & 3) * 8;
+                        const s4v w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v *)at);
+                        const uint2 u = __builtin_bit_cast(uint2, w);
+                        v[2 * k] = u.x;
+                        v[2 * k + 1] = u.y;
+                    }
+#pragma unroll
+                    for (int x = 0; x < RT; x++) o[x][d] = Mma<T>::dot(v, lo[x], Mma<T>::dot(v, hi[x], o[x][d]));
                 } else {
-                    at = id * p.page_stride + (j - pi * p.page.d) * p.token_stride + kvh * p.head_stride;
-                    const T *k = (const T *)p.kc + at;
-                    z = 0.0f;
-                    for (int e = 0; e < D; e++) z = fmaf(sq[e], fw_to_f32(k[e]), z);
-                    z *= p.scale;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float v = *(const float *)(vt + (4 * c + i) * VROW + d * 64 + lr * 4);
+#pragma unroll
+                        for (int x = 0; x < RT; x++)
+                            o[x][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, pw[x][i], o[x][d], 0, 0, 0);
+                    }
                 }
             }
-            if (!__any(sees)) continue;
-            any = true;
-            const float mn = fmaxf(m, fw_wave_max(z)); // NaN scores come back in e^(z - m)
-            const float base = mn == -INFINITY ? 0.0f : mn;
-            const float e = sees ? expf(z - base) : 0.0f, f = expf(m - base);
-            l = l * f + fw_wave_sum(e);
-            m = mn;
-            sp[lane] = e;
-            sat[lane] = sees ? at : -2;
-            __syncthreads();
-            for (int x = 0; x < D / 64; x++) {
-                float acc = o[x] * f;
-                for (int t = 0; t < 64; t++) {
-                    if (sat[t] < -1) continue;
-                    acc = fmaf(sp[t], sat[t] < 0 ? 0.0f : fw_to_f32(((const T *)p.vc)[sat[t] + x * 64 + lane]), acc);
+            if (careful) {
+                // the values that were dropped, for the rows that see them
+                for (int key = 0; key < KEYS; key++) {
+                    const int from = (key & 15) >> 2, slot = (key >> 4) * 4 + (key & 3);
+                    const int64_t there = __shfl(key < 16 ? here[0] : here[KT - 1], key & 15);
+                    if (there < 0) continue;
+                    for (int x = 0; x < RT; x++) {
+                        float w = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 4 * KT; i++) w = i == slot ? pw[x][i] : w;
+                        w = __shfl(w, from * 16 + lr);
+                        const bool yes = __shfl((int)sees[x], from * 16 + lr) >> slot & 1;
+#pragma unroll
+                        for (int d = 0; d < DT; d++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const float v = fw_to_f32(((const T *)p.vc)[there + 16 * d + 4 * c + i]);
+                                if (yes && !(fabsf(v) < INFINITY)) o[x][d][i] += w * v;
+                            }
+                    }
                 }
-                o[x] = acc;
             }
-            __syncthreads();
         }
-        for (int x = 0; x < D / 64; x++) out[x * 64 + lane] = fw_cvt<T>(any ? o[x] / l : 0.0f);
+        // Outputs that are not finite may come from values a row does not see
+        // (0 times infinity) or from the halves of a weight (infinity less
+        // infinity): then once more, with such values taken row by row.
+        bool odd = false;
+#pragma unroll
+        for (int x = 0; x < RT; x++)
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) odd |= !(fabsf(o[x][d][i]) < INFINITY);
+        if (!__any(odd)) break;
+    }
+
+    // join the waves: weights of the common maximum, outputs added up wave by wave
+#pragma unroll
+    for (int x = 0; x < RT; x++) {
+        l[x] = quarters_sum(l[x]);
+        if (c == 0) {
+            sm[wave][x * 16 + lr] = m[x];
+            sl[wave][x * 16 + lr] = l[x];
+        }
+    }
+    __syncthreads();
+    float f[RT];
+#pragma unroll
+    for (int x = 0; x < RT; x++) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; w++) mx = fmaxf(mx, sm[w][x * 16 + lr]);
+        f[x] = __builtin_amdgcn_exp2f(m[x] - TREE_BIAS - tree_base(mx));
+        l[x] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+            l[x] = fmaf(__builtin_amdgcn_exp2f(sm[w][x * 16 + lr] - TREE_BIAS - tree_base(mx)), sl[w][x * 16 + lr], l[x]);
+        m[x] = mx;
+    }
+    float *ot = (float *)lds;
+    for (int w = 3; w >= 0; w--) {
+        if (wave == w) {
+#pragma unroll
+            for (int x = 0; x < RT; x++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    f4 *at = (f4 *)(ot + (x * 16 + lr) * D + ((16 * d + 4 * c) ^ (4 * (lr & 7))));
+                    const f4 mine = f[x] == 0.0f ? f4{} : o[x][d] * f[x];
+                    o[x][d] = w == 3 ? mine : mine + *at;
+                    if (w) *at = o[x][d];
+                }
+        }
+        __syncthreads();
+    }
+    if (wave) return;
+    // wave 0 holds the sums
+#pragma unroll
+    for (int x = 0; x < RT; x++) {
+        const int t = t0 + x * 16 + lr;
+        if (t >= total) continue;
+        if (whole) {
+            T *out = (T *)p.out + (int64_t)(rq.row0 + node[x]) * p.out_row + qat[x] * p.out_head + 4 * c;
+            const bool any = tree_sees_any(p, rq, node[x]);
+            const float inv = 1.0f / l[x]; // l = 0: 0 / 0 below
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                f4 v = l[x] == 0.0f ? f4{} + __builtin_nanf("") : o[x][d] * inv;
+                if (!any) v = f4{};
+                *(typename Vec4<T>::type *)(out + 16 * d) = pack4<T>(v);
+            }
+        } else {
+            const int64_t slot = (((int64_t)r * p.tiles + tile) * p.kv_heads + kvh) * p.splits + split;
+            float *at = p.parts + (slot * (RT * 16) + x * 16 + lr) * (D + 4);
+#pragma unroll
+            for (int d = 0; d < DT; d++) *(f4 *)(at + 16 * d + 4 * c) = o[x][d];
+            if (c == 0) {
+                at[D] = m[x];
+                at[D + 1] = l[x];
+            }
+        }
     }
 }
 
+// The parts of a request's chunks into its outputs: a wave per row and head.
 template <typename T, int D>
-static void tree_launch(hipStream_t st, const TreeP &p) {
-    hipLaunchKernelGGL((k_tree_attn<T, D>), dim3((unsigned)std::min(p.max_new, 65535), p.heads, p.n_req), dim3(64), 0,
-                       st, p);
+__global__ void __launch_bounds__(256) k_tree_join(TreeP p) {
+    const int lane = threadIdx.x & 63, r = blockIdx.z, h = blockIdx.y;
+    const TreeReq rq = tree_req(p, r);
+    const int group = p.heads / p.kv_heads, kvh = h / group;
+    for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < rq.n; i += gridDim.x * 4) {
+        const int t = i * group + h % group, tile = t / p.tile_rows;
+        const int keys = rq.bad ? 0 : p.words ? rq.len + rq.n
+            : min(rq.len + rq.n, rq.len + (min((tile + 1) * p.tile_rows, rq.n * group) - 1) / group + 1);
+        const int parts = (keys + p.chunk - 1) / p.chunk;
+        const int64_t slot = (((int64_t)r * p.tiles + tile) * p.kv_heads + kvh) * p.splits;
+        const float *at = p.parts + (slot * p.tile_rows + t % p.tile_rows) * (D + 4);
+        const int64_t step = (int64_t)p.tile_rows * (D + 4);
+        float mx = -INFINITY;
+        for (int s = 0; s < parts; s++) mx = fmaxf(mx, at[s * step + D]);
+        float l = 0.0f, o[D / 64] = {};
+        for (int s = 0; s < parts; s++) {
+            const float f = __builtin_amdgcn_exp2f(at[s * step + D] - TREE_BIAS - tree_base(mx));
+            l = fmaf(f, at[s * step + D + 1], l);
+            for (int x = 0; x < D / 64; x++) o[x] = fmaf(f, at[s * step + x * 64 + lane], o[x]);
+        }
+        T *out = (T *)p.out + (int64_t)(rq.row0 + i) * p.out_row + (int64_t)h * p.out_head;
+        const bool any = rq.bad || tree_sees_any(p, rq, i);
+        for (int x = 0; x < D / 64; x++)
+            out[x * 64 + lane] = fw_cvt<T>(!any ? 0.0f : l == 0.0f ? __builtin_nanf("") : o[x] / l);
+    }
+}
+
+// How a call of these sizes is cut.  Blocks of 16, 32 or 64 rows, so that the
+// rows of a small tree fill their tiles (f32 rows take twice the registers: 32
+// at most); the keys are split until TREE_BLOCKS blocks are there, but not into
+// chunks below TREE_CHUNK keys.
+#define TREE_BLOCKS 768
+#define TREE_CHUNK 256
+struct TreeCut {
+    int rt, splits, chunk;
+    int64_t tiles;
+    uint64_t bytes;
+};
+static TreeCut tree_cut(int32_t n_req, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_new,
+                        int32_t max_len, bool f32) {
+    TreeCut t;
+    const int64_t rows = (int64_t)max_new * (n_heads / n_kv_heads);
+    t.rt = rows <= 16 ? 1 : rows <= 32 || f32 ? 2 : 4;
+    t.tiles = (rows + 16 * t.rt - 1) / (16 * t.rt);
+    const int64_t base = std::max<int64_t>(1, (int64_t)n_req * n_kv_heads * t.tiles);
+    const int64_t most = std::max<int64_t>(1, ((int64_t)max_len + TREE_CHUNK - 1) / TREE_CHUNK);
+    const int64_t want = std::max<int64_t>(1, std::min(most, TREE_BLOCKS / base));
+    t.chunk = (int)((((int64_t)max_len + want - 1) / want + 127) / 128 * 128);
+    t.chunk = std::max(t.chunk, 128);
+    t.splits = (int)std::max<int64_t>(1, ((int64_t)max_len + t.chunk - 1) / t.chunk);
+    // enough for every smaller call too
+    t.bytes = most > 1 ? (uint64_t)std::min<int64_t>(TREE_BLOCKS, base * most) * (16 * t.rt) * (head_dim + 4) * 4 : 0;
+    return t;
+}
+
+template <typename T, int D, int RT>
+static void tree_go(hipStream_t st, const TreeP &p, int n_req) {
+    hipLaunchKernelGGL((k_tree_attn<T, D, RT>), dim3(p.splits, p.kv_heads * p.tiles, n_req), dim3(256), 0, st, p);
+    if (p.splits > 1)
+        hipLaunchKernelGGL((k_tree_join<T, D>), dim3((unsigned)((std::min(p.max_new, 4096) + 3) / 4), p.heads, n_req),
+                           dim3(256), 0, st, p);
+}
+template <typename T, int D>
+static void tree_rows(hipStream_t st, const TreeP &p, int n_req, int rt) {
+    if (rt == 1) tree_go<T, D, 1>(st, p, n_req);
+    else if (rt == 2) tree_go<T, D, 2>(st, p, n_req);
+    else if constexpr (sizeof(T) == 2) tree_go<T, D, 4>(st, p, n_req);
 }
 template <typename T>
-static void tree_dim(hipStream_t st, int d, const TreeP &p) {
-    if (d == 64) tree_launch<T, 64>(st, p);
-    else tree_launch<T, 128>(st, p);
+static void tree_dim(hipStream_t st, int d, const TreeP &p, int n_req, int rt) {
+    if (d == 64) tree_rows<T, 64>(st, p, n_req, rt);
+    else tree_rows<T, 128>(st, p, n_req, rt);
 }
 
 extern "C" fwhip_status fwhip_tree_attn_workspace(int32_t n_req, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
@@ -111,7 +580,9 @@ extern "C" fwhip_status fwhip_tree_attn_workspace(int32_t n_req, int32_t n_heads
         return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn_workspace: bad size");
     if (head_dim != 64 && head_dim != 128)
         return fw_fail(FWHIP_ERR_UNSUPPORTED, "fwhip_tree_attn_workspace: head_dim must be 64 or 128");
-    *bytes = 0;
+    // the type is not asked for: whichever cut needs more
+    *bytes = std::max(tree_cut(n_req, n_heads, n_kv_heads, head_dim, max_new, max_len, false).bytes,
+                      tree_cut(n_req, n_heads, n_kv_heads, head_dim, max_new, max_len, true).bytes);
     return FWHIP_OK;
 }
 
@@ -136,6 +607,7 @@ extern "C" fwhip_status fwhip_tree_attn(fwhip_ctx *c, const fwhip_tree_attn_args
     if (a->n_req && a->n_rows) {
         if (!a->q || !a->out || !a->len || !a->row_start || !a->table || (a->n_pages && (!a->k_cache || !a->v_cache)))
             return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn: NULL argument");
+        if (a->n_pages < 1) return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn: a cache of no pages");
         const int eb = fw_dtype_bytes(a->dtype);
         if (!fw_aligned(a->q, 16) || !fw_aligned(a->k_cache, 16) || !fw_aligned(a->v_cache, 16) || !fw_aligned(a->out, 16))
             return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn: q, the caches and out must be 16-byte aligned");
@@ -184,8 +656,17 @@ extern "C" fwhip_status fwhip_tree_attn(fwhip_ctx *c, const fwhip_tree_attn_args
     p.row_start = a->row_start;
     p.mask = a->mask;
     p.out = a->out;
-    if (a->dtype == FWHIP_T_F32) tree_dim<float>(c->stream, a->head_dim, p);
-    else if (a->dtype == FWHIP_T_F16) tree_dim<fw_f16>(c->stream, a->head_dim, p);
-    else tree_dim<fw_bf16>(c->stream, a->head_dim, p);
+    const TreeCut cut = tree_cut(a->n_req, a->n_heads, a->n_kv_heads, a->head_dim, std::min(a->max_new, a->n_rows), a->max_len,
+                                 a->dtype == FWHIP_T_F32);
+    if (cut.tiles * a->n_kv_heads > 65535)
+        return fw_fail(FWHIP_ERR_UNSUPPORTED, "fwhip_tree_attn: more than 65535 row tiles x K/V heads");
+    p.tiles = (int)cut.tiles;
+    p.splits = cut.splits;
+    p.chunk = cut.chunk;
+    p.tile_rows = 16 * cut.rt;
+    p.parts = (float *)a->workspace;
+    if (a->dtype == FWHIP_T_F32) tree_dim<float>(c->stream, a->head_dim, p, a->n_req, cut.rt);
+    else if (a->dtype == FWHIP_T_F16) tree_dim<fw_f16>(c->stream, a->head_dim, p, a->n_req, cut.rt);
+    else tree_dim<fw_bf16>(c->stream, a->head_dim, p, a->n_req, cut.rt);
     return fw_launched("fwhip_tree_attn");
 }

@@ -444,7 +444,8 @@ def test_attention_offsets_past_32_bits(tctx):
     table = ids.to(torch.int32).view(1, n).cuda()
     out = torch.empty_like(s["q"]).cuda()
     ops.tree_attn(tctx, s["q"].cuda(), kc, vc, table, dev(s["lens"]), dev(s["row_start"]), out, scale=s["scale"],
-                  max_new=6, mask=dev(s["mask"].astype(np.int64)))
+                  max_new=6, mask=dev(s["mask"].astype(np.int64)),
+                  workspace=torch.empty(ops.tree_attn_workspace(1, 16, kv, dim, 6, n * page) + 16, dtype=torch.uint8).cuda())
     close(out, want, tol)
     # the same slots written by append
     kc[total - 1] = 0
