@@ -47,7 +47,8 @@ struct Mma<fw_f16> {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
     }
     // p = hi + lo up to 2^-20 of p: two f16 of 11 bits each, cut
-    static __device__ __forceinline__ void split(const float *p, u4 &hi, u4 &lo) {
+    static __device__ __forceinline__ void split(const f4 (&w)[2], u4 &hi, u4 &lo) {
+        const float p[8] = {w[0][0], w[0][1], w[0][2], w[0][3], w[1][0], w[1][1], w[1][2], w[1][3]};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const auto h = __builtin_amdgcn_cvt_pkrtz(p[2 * i], p[2 * i + 1]);
@@ -64,7 +65,8 @@ struct Mma<fw_bf16> {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
     }
     // p = hi + lo up to 2^-16 of p: the upper half of the f32, and the rest rounded to 8 bits
-    static __device__ __forceinline__ void split(const float *p, u4 &hi, u4 &lo) {
+    static __device__ __forceinline__ void split(const f4 (&w)[2], u4 &hi, u4 &lo) {
+        const float p[8] = {w[0][0], w[0][1], w[0][2], w[0][3], w[1][0], w[1][1], w[1][2], w[1][3]};
         typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -110,19 +112,6 @@ __device__ __forceinline__ void wave_fence() {
 #define TREE_BIAS 15.0f
 __device__ __forceinline__ float tree_base(float m) { return m == -INFINITY ? 0.0f : m - TREE_BIAS; }
 
-template <typename T>
-__device__ __forceinline__ bool has_nonfinite(u4 v) {
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if constexpr (sizeof(T) == 4) bad |= (v[i] & 0x7f800000u) == 0x7f800000u;
-        else {
-            constexpr uint32_t E = std::is_same<T, fw_f16>::value ? 0x7c00u : 0x7f80u;
-            bad |= (v[i] & E) == E || (v[i] >> 16 & E) == E;
-        }
-    }
-    return bad;
-}
 template <typename T>
 __device__ __forceinline__ u4 drop_nonfinite(u4 v) {
 #pragma unroll
@@ -177,62 +166,30 @@ __device__ __forceinline__ typename Vec4<T>::type pack4(f4 v) {
                           fw_cvt<T>(v[2]).b | (uint32_t)fw_cvt<T>(v[3]).b << 16);
 }
 
-// A block: one K/V head of one request, RT * 16 of its query rows (new token x
-// query head of the group), and one chunk of its keys.  Its four waves take the
-// chunk's steps of KT * 16 keys in turn, each with a running maximum, sum and
-// output of its own for all rows, so K and V are read once a block; they are
-// joined through LDS at the end.  A wave's K tile goes from memory to the lanes
-// that multiply it; its V tile passes through LDS, where the transposing read
-// gives each lane the keys of one feature.  The next step's tiles are in flight
-// while a step computes.
+// ---------------------------------------------------------------------------
+// What both kernels below do with a wave's rows: RT tiles of 16 query rows (new
+// token x query head of the K/V head's group), and steps of KEYS keys.
 template <typename T, int D, int RT>
-__global__ void __launch_bounds__(256, RT == 4 ? 1 : 2) k_tree_attn(TreeP p) {
-    constexpr int KT = Mma<T>::KT, KEYS = 16 * KT, NS = D * (int)sizeof(T) / 64, DT = D / 16;
-    constexpr int VROW = D * (int)sizeof(T) + 32; // bytes of a V row in LDS: rows 8 banks apart
-    constexpr int VBYTES = 4 * KEYS * VROW, OBYTES = RT * 16 * D * 4;
-    __shared__ __attribute__((aligned(16))) char lds[VBYTES > OBYTES ? VBYTES : OBYTES];
-    __shared__ float sm[4][RT * 16], sl[4][RT * 16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4;
-    const int group = p.heads / p.kv_heads;
-    const int split = blockIdx.x, kvh = blockIdx.y % p.kv_heads, tile = blockIdx.y / p.kv_heads, r = blockIdx.z;
-    const TreeReq rq = tree_req(p, r);
-    const bool whole = p.splits == 1;
-    if (rq.bad) { // may have more rows than there are tiles
-        if (whole && tile == 0)
-            for (int64_t e = threadIdx.x; e < (int64_t)rq.n * group * D; e += 256) {
-                const int64_t i = e / D / group, h = kvh * group + e / D % group;
-                ((T *)p.out)[(rq.row0 + i) * p.out_row + h * p.out_head + e % D] = fw_cvt<T>(__builtin_nanf(""));
-            }
-        return;
-    }
-    const int total = rq.n * group, t0 = tile * RT * 16;
-    if (t0 >= total) return;
-    const int end = rq.len + rq.n; // keys of the request
-    // a chain's rows see no further than the tile's last token
-    const int tile_end = p.words ? end : min(end, rq.len + (min(t0 + RT * 16, total) - 1) / group + 1);
-    const int first = split * p.chunk, last = min(tile_end, first + p.chunk);
-    if (!whole && first >= tile_end) return; // the join reads no part of it
-
-    // query rows
-    int node[RT];
-    int64_t qat[RT];
+struct Rows {
+    static constexpr int KT = Mma<T>::KT, KEYS = 16 * KT, NS = D * (int)sizeof(T) / 64, DT = D / 16;
+    int node[RT], head[RT]; // of row lr of each tile
     u4 q[RT][NS];
-#pragma unroll
-    for (int x = 0; x < RT; x++) {
-        const int t = min(t0 + x * 16 + lr, total - 1);
-        node[x] = t / group;
-        qat[x] = (int64_t)(kvh * group + t % group);
-        const T *at = (const T *)p.q + (int64_t)(rq.row0 + node[x]) * p.q_row + qat[x] * p.q_head;
-#pragma unroll
-        for (int s = 0; s < NS; s++) q[x][s] = *(const u4 *)((const char *)at + s * 64 + c * 16);
-    }
-    const float zs = p.scale * 1.44269504088896340736f; // scores in base 2
-    char *vt = lds + wave * KEYS * VROW;
-    const int32_t *trow = p.table + (int64_t)r * p.table_stride;
-
     f4 o[RT][DT];
     float m[RT], l[RT];
-    for (int careful = 0; careful < 2; careful++) {
+
+    __device__ __forceinline__ void load(const TreeP &p, const TreeReq &rq, int t0, int total, int kvh, int group) {
+        const int lane = threadIdx.x & 63, lr = lane & 15, c = lane >> 4;
+#pragma unroll
+        for (int x = 0; x < RT; x++) {
+            const int t = min(t0 + x * 16 + lr, total - 1); // the last row again behind the end
+            node[x] = t / group;
+            head[x] = kvh * group + t % group;
+            const T *at = (const T *)p.q + (int64_t)(rq.row0 + node[x]) * p.q_row + head[x] * p.q_head;
+#pragma unroll
+            for (int s = 0; s < NS; s++) q[x][s] = *(const u4 *)((const char *)at + s * 64 + c * 16);
+        }
+    }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int x = 0; x < RT; x++) {
             m[x] = -INFINITY;
@@ -240,261 +197,443 @@ __global__ void __launch_bounds__(256, RT == 4 ? 1 : 2) k_tree_attn(TreeP p) {
 #pragma unroll
             for (int d = 0; d < DT; d++) o[x][d] = f4{};
         }
-        int j0 = first + wave * KEYS;
-        int pid[KT];        // the next step's pages
-        int64_t off[KT];    // this step's keys, -1 where there is none
-        u4 kf[KT][NS], vf[KT][NS];
-        auto pages = [&](int j) {
+    }
+    // Scores of the step at key j to -inf where a row does not see the key; the
+    // keys it sees as bits (4 per key tile).
+    __device__ __forceinline__ uint32_t mask(const TreeP &p, const TreeReq &rq, int x, int j, int last, f4 (&z)[KT]) const {
+        const int c = (threadIdx.x & 63) >> 4;
+        uint32_t sees = 0;
 #pragma unroll
-            for (int k = 0; k < KT; k++) {
-                const int key = j + k * 16 + lr;
-                pid[k] = key < last ? trow[fw_div((uint32_t)key, p.page)] : -1;
+        for (int k = 0; k < KT; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int key = j + k * 16 + 4 * c + i, t = key - rq.len;
+                bool yes = key < last;
+                if (yes && t >= 0)
+                    yes = p.words ? p.mask[(int64_t)(rq.row0 + node[x]) * p.words + (t >> 6)] >> (t & 63) & 1 : t <= node[x];
+                if (!yes) z[k][i] = -INFINITY;
+                sees |= (uint32_t)yes << (4 * k + i);
             }
-        };
-        auto offsets = [&](int j) {
+        return sees;
+    }
+    // Scores to weights (in place); what is there already is scaled to the new maximum.
+    __device__ __forceinline__ void weigh(int x, f4 (&z)[KT]) {
+        float mx = z[0][0];
 #pragma unroll
-            for (int k = 0; k < KT; k++) {
-                const uint32_t key = (uint32_t)(j + k * 16 + lr), pi = fw_div(key, p.page);
-                off[k] = (uint32_t)pid[k] < (uint32_t)p.n_pages
-                             ? (int64_t)pid[k] * p.page_stride + (int64_t)(key - pi * p.page.d) * p.token_stride +
-                                   (int64_t)kvh * p.head_stride
-                             : -1;
-            }
-        };
-        auto load = [&](const void *base, u4 (*f)[NS]) {
+        for (int k = 0; k < KT; k++)
 #pragma unroll
-            for (int k = 0; k < KT; k++) {
-                const char *at = (const char *)((const T *)base + max(off[k], (int64_t)0)) + c * 16;
+            for (int i = 0; i < 4; i++) mx = fmaxf(mx, z[k][i]);
+        mx = quarters_max(mx);
+        if (__any(mx > m[x])) {
+            const float mn = fmaxf(mx, m[x]), f = __builtin_amdgcn_exp2f(m[x] - TREE_BIAS - tree_base(mn));
+            m[x] = mn;
+            l[x] *= f;
 #pragma unroll
-                for (int s = 0; s < NS; s++) f[k][s] = *(const u4 *)(at + s * 64);
-            }
-        };
-        if (j0 < last) {
-            pages(j0);
-            offsets(j0);
-            load(p.kc, kf);
-            load(p.vc, vf);
-            pages(j0 + 4 * KEYS);
+            for (int d = 0; d < DT; d++) o[x][d] *= f;
         }
-        for (; j0 < last; j0 += 4 * KEYS) {
-            int64_t here[KT];
+        const float base = tree_base(m[x]);
 #pragma unroll
-            for (int k = 0; k < KT; k++) here[k] = off[k];
-            // scores of this step: keys 16 k + 4 c + 0..3 of row lr
-            f4 z[RT][KT];
+        for (int k = 0; k < KT; k++)
 #pragma unroll
-            for (int x = 0; x < RT; x++)
+            for (int i = 0; i < 4; i++) {
+                z[k][i] = __builtin_amdgcn_exp2f(z[k][i] - base);
+                l[x] += z[k][i];
+            }
+    }
+    // o += weights times the V tile in LDS (rows of VROW bytes).
+    template <int VROW>
+    __device__ __forceinline__ void add(const char *vt, const f4 (&w)[RT][KT]) {
+        const int lane = threadIdx.x & 63, lr = lane & 15, c = lane >> 4;
+        u4 hi[RT], lo[RT];
+        if constexpr (sizeof(T) == 2)
 #pragma unroll
-                for (int k = 0; k < KT; k++) {
-                    f4 a = {};
+            for (int x = 0; x < RT; x++) Mma<T>::split(w[x], hi[x], lo[x]);
 #pragma unroll
-                    for (int s = 0; s < NS; s++) a = Mma<T>::dot(kf[k][s], q[x][s], a);
-                    z[x][k] = a * zs;
+        for (int d = 0; d < DT; d++) {
+            if constexpr (sizeof(T) == 2) {
+                u4 v;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const char *at = vt + (k * 16 + 4 * c + (lr >> 2)) * VROW + d * 32 + (lr & 3) * 8;
+                    const uint2 u = __builtin_bit_cast(
+                        uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v *)at));
+                    v[2 * k] = u.x;
+                    v[2 * k + 1] = u.y;
                 }
-            const bool edge = j0 + KEYS > min(rq.len, last); // new tokens, or the chunk's end
-            const bool lost = __any(here[0] < 0 || here[KT - 1] < 0); // beyond the end, or no page
-            if (lost) {
 #pragma unroll
-                for (int k = 0; k < KT; k++)
-                    if (here[k] < 0)
+                for (int x = 0; x < RT; x++) o[x][d] = Mma<T>::dot(v, lo[x], Mma<T>::dot(v, hi[x], o[x][d]));
+            } else {
 #pragma unroll
-                        for (int s = 0; s < NS; s++) vf[k][s] = u4{};
-            }
-            if (careful) {
+                for (int i = 0; i < 4; i++) {
+                    const float v = *(const float *)(vt + (4 * c + i) * VROW + d * 64 + lr * 4);
 #pragma unroll
-                for (int k = 0; k < KT; k++)
-#pragma unroll
-                    for (int s = 0; s < NS; s++) vf[k][s] = drop_nonfinite<T>(vf[k][s]);
-            }
-            wave_fence();
-#pragma unroll
-            for (int k = 0; k < KT; k++)
-#pragma unroll
-                for (int s = 0; s < NS; s++) *(u4 *)(vt + (k * 16 + lr) * VROW + s * 64 + c * 16) = vf[k][s];
-            wave_fence();
-            if (j0 + 4 * KEYS < last) {
-                offsets(j0 + 4 * KEYS);
-                load(p.kc, kf);
-                load(p.vc, vf);
-                pages(j0 + 8 * KEYS);
-            }
-            uint32_t sees[RT];
-#pragma unroll
-            for (int x = 0; x < RT; x++) sees[x] = 0xffffffffu;
-            if (edge || lost) {
-#pragma unroll
-                for (int x = 0; x < RT; x++) {
-                    sees[x] = 0;
-#pragma unroll
-                    for (int k = 0; k < KT; k++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int key = j0 + k * 16 + 4 * c + i, t = key - rq.len;
-                            bool yes = key < last;
-                            if (yes && t >= 0)
-                                yes = p.words ? p.mask[(int64_t)(rq.row0 + node[x]) * p.words + (t >> 6)] >> (t & 63) & 1
-                                              : t <= node[x];
-                            // a key whose table entry is no page makes its rows NaN
-                            const int64_t there = __shfl(here[k], 4 * c + i);
-                            z[x][k][i] = !yes ? -INFINITY : there < 0 ? __builtin_nanf("") : z[x][k][i];
-                            sees[x] |= (uint32_t)yes << (4 * k + i);
-                        }
+                    for (int x = 0; x < RT; x++)
+                        o[x][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, w[x][0][i], o[x][d], 0, 0, 0);
                 }
             }
-            // weights
-            u4 hi[RT], lo[RT];
-            float pw[RT][4 * KT];
+        }
+    }
+    // The values of V that are not finite, for the rows that see them (they were
+    // left out of the tile).
+    __device__ __forceinline__ void add_dropped(const TreeP &p, const int32_t *trow, int kvh, int j, int last,
+                                             const f4 (&w)[RT][KT], const uint32_t (&sees)[RT]) {
+        const int lane = threadIdx.x & 63, lr = lane & 15, c = lane >> 4;
+        for (int key = 0; key < KEYS && j + key < last; key++) {
+            const int from = ((key & 15) >> 2) * 16 + lr, slot = (key >> 4) * 4 + (key & 3);
+            const uint32_t pi = fw_div((uint32_t)(j + key), p.page);
+            const int32_t id = trow[pi];
+            if ((uint32_t)id >= (uint32_t)p.n_pages) continue;
+            const T *v = (const T *)p.vc + id * p.page_stride + (int64_t)(j + key - pi * p.page.d) * p.token_stride +
+                         kvh * p.head_stride;
 #pragma unroll
             for (int x = 0; x < RT; x++) {
-                float mx = z[x][0][0];
+                float mine = 0.0f;
 #pragma unroll
-                for (int k = 0; k < KT; k++)
+                for (int i = 0; i < 4 * KT; i++) mine = i == slot ? w[x][i >> 2][i & 3] : mine;
+                mine = __shfl(mine, from);
+                const bool yes = __shfl((int)sees[x], from) >> slot & 1;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) mx = fmaxf(mx, z[x][k][i]);
-                mx = quarters_max(mx);
-                if (__any(mx > m[x])) {
-                    const float mn = fmaxf(mx, m[x]), f = __builtin_amdgcn_exp2f(m[x] - TREE_BIAS - tree_base(mn));
-                    m[x] = mn;
-                    l[x] *= f;
-#pragma unroll
-                    for (int d = 0; d < DT; d++) o[x][d] *= f;
-                }
-                const float base = tree_base(m[x]);
-#pragma unroll
-                for (int k = 0; k < KT; k++)
+                for (int d = 0; d < DT; d++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        pw[x][4 * k + i] = __builtin_amdgcn_exp2f(z[x][k][i] - base);
-                        l[x] += pw[x][4 * k + i];
+                        const float a = fw_to_f32(v[16 * d + 4 * c + i]);
+                        if (yes && !(fabsf(a) < INFINITY)) o[x][d][i] += mine * a;
                     }
-                if constexpr (sizeof(T) == 2) Mma<T>::split(pw[x], hi[x], lo[x]);
-            }
-            // outputs: features 16 d + 4 c + 0..3 of row lr
-#pragma unroll
-            for (int d = 0; d < DT; d++) {
-                if constexpr (sizeof(T) == 2) {
-                    u4 v;
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const char *at = vt + (k * 16 + 4 * c + (lr >> 2)) * VROW + d * 32 + (lr & 3) * 8;
-                        const s4v w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v *)at);
-                        const uint2 u = __builtin_bit_cast(uint2, w);
-                        v[2 * k] = u.x;
-                        v[2 * k + 1] = u.y;
-                    }
-#pragma unroll
-                    for (int x = 0; x < RT; x++) o[x][d] = Mma<T>::dot(v, lo[x], Mma<T>::dot(v, hi[x], o[x][d]));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float v = *(const float *)(vt + (4 * c + i) * VROW + d * 64 + lr * 4);
-#pragma unroll
-                        for (int x = 0; x < RT; x++)
-                            o[x][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, pw[x][i], o[x][d], 0, 0, 0);
-                    }
-                }
-            }
-            if (careful) {
-                // the values that were dropped, for the rows that see them
-                for (int key = 0; key < KEYS; key++) {
-                    const int from = (key & 15) >> 2, slot = (key >> 4) * 4 + (key & 3);
-                    const int64_t there = __shfl(key < 16 ? here[0] : here[KT - 1], key & 15);
-                    if (there < 0) continue;
-                    for (int x = 0; x < RT; x++) {
-                        float w = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 4 * KT; i++) w = i == slot ? pw[x][i] : w;
-                        w = __shfl(w, from * 16 + lr);
-                        const bool yes = __shfl((int)sees[x], from * 16 + lr) >> slot & 1;
-#pragma unroll
-                        for (int d = 0; d < DT; d++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const float v = fw_to_f32(((const T *)p.vc)[there + 16 * d + 4 * c + i]);
-                                if (yes && !(fabsf(v) < INFINITY)) o[x][d][i] += w * v;
-                            }
-                    }
-                }
             }
         }
-        // Outputs that are not finite may come from values a row does not see
-        // (0 times infinity) or from the halves of a weight (infinity less
-        // infinity): then once more, with such values taken row by row.
-        bool odd = false;
+    }
+    __device__ __forceinline__ bool odd() const {
+        bool any = false;
 #pragma unroll
         for (int x = 0; x < RT; x++)
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) odd |= !(fabsf(o[x][d][i]) < INFINITY);
-        if (!__any(odd)) break;
+                for (int i = 0; i < 4; i++) any |= !(fabsf(o[x][d][i]) < INFINITY);
+        return any;
     }
-
-    // join the waves: weights of the common maximum, outputs added up wave by wave
+    // One result of `parts` waves that took different keys of the same rows: the
+    // first one gets it.  sm / sl: [parts][rows], ot: [rows][D] in LDS; every
+    // thread of the block comes here.
+    __device__ __forceinline__ void join(int part, int parts, int row0, int rows, float *sm, float *sl, float *ot) {
+        const int lane = threadIdx.x & 63, lr = lane & 15, c = lane >> 4;
+        float f[RT];
 #pragma unroll
-    for (int x = 0; x < RT; x++) {
-        l[x] = quarters_sum(l[x]);
-        if (c == 0) {
-            sm[wave][x * 16 + lr] = m[x];
-            sl[wave][x * 16 + lr] = l[x];
+        for (int x = 0; x < RT; x++)
+            if (c == 0) {
+                sm[part * rows + row0 + x * 16 + lr] = m[x];
+                sl[part * rows + row0 + x * 16 + lr] = l[x];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < RT; x++) {
+            const float *am = sm + row0 + x * 16 + lr, *al = sl + row0 + x * 16 + lr;
+            float mx = -INFINITY;
+            for (int w = 0; w < parts; w++) mx = fmaxf(mx, am[w * rows]);
+            f[x] = __builtin_amdgcn_exp2f(m[x] - TREE_BIAS - tree_base(mx));
+            l[x] = 0.0f;
+            for (int w = 0; w < parts; w++)
+                l[x] = fmaf(__builtin_amdgcn_exp2f(am[w * rows] - TREE_BIAS - tree_base(mx)), al[w * rows], l[x]);
+            m[x] = mx;
+        }
+        for (int w = parts - 1; w >= 0; w--) {
+            if (part == w) {
+#pragma unroll
+                for (int x = 0; x < RT; x++)
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        f4 *at = (f4 *)(ot + (row0 + x * 16 + lr) * D + ((16 * d + 4 * c) ^ (4 * (lr & 7))));
+                        const f4 mine = f[x] == 0.0f ? f4{} : o[x][d] * f[x];
+                        o[x][d] = w == parts - 1 ? mine : mine + *at;
+                        if (w) *at = o[x][d];
+                    }
+            }
+            __syncthreads();
         }
     }
-    __syncthreads();
-    float f[RT];
+    // Rows t0 + 0..16 RT - 1 of the tile of R rows that begins at tile0: outputs, or this chunk's part.
+    __device__ __forceinline__ void store(const TreeP &p, const TreeReq &rq, int r, int tile, int split, int kvh, int t0,
+                                          int total, bool whole) {
+        const int lane = threadIdx.x & 63, lr = lane & 15, c = lane >> 4;
 #pragma unroll
-    for (int x = 0; x < RT; x++) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < 4; w++) mx = fmaxf(mx, sm[w][x * 16 + lr]);
-        f[x] = __builtin_amdgcn_exp2f(m[x] - TREE_BIAS - tree_base(mx));
-        l[x] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; w++)
-            l[x] = fmaf(__builtin_amdgcn_exp2f(sm[w][x * 16 + lr] - TREE_BIAS - tree_base(mx)), sl[w][x * 16 + lr], l[x]);
-        m[x] = mx;
-    }
-    float *ot = (float *)lds;
-    for (int w = 3; w >= 0; w--) {
-        if (wave == w) {
-#pragma unroll
-            for (int x = 0; x < RT; x++)
+        for (int x = 0; x < RT; x++) {
+            const int t = t0 + x * 16 + lr;
+            if (t >= total) continue;
+            if (whole) {
+                T *out = (T *)p.out + (int64_t)(rq.row0 + node[x]) * p.out_row + head[x] * p.out_head + 4 * c;
+                const bool any = tree_sees_any(p, rq, node[x]);
+                const float inv = 1.0f / l[x];
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
-                    f4 *at = (f4 *)(ot + (x * 16 + lr) * D + ((16 * d + 4 * c) ^ (4 * (lr & 7))));
-                    const f4 mine = f[x] == 0.0f ? f4{} : o[x][d] * f[x];
-                    o[x][d] = w == 3 ? mine : mine + *at;
-                    if (w) *at = o[x][d];
+                    f4 v = l[x] == 0.0f ? f4{} + __builtin_nanf("") : o[x][d] * inv; // 0 / 0: every key scored -inf
+                    if (!any) v = f4{};
+                    *(typename Vec4<T>::type *)(out + 16 * d) = pack4<T>(v);
                 }
+            } else {
+                const int64_t slot = (((int64_t)r * p.tiles + tile) * p.kv_heads + kvh) * p.splits + split;
+                float *at = p.parts + (slot * p.tile_rows + t - tile * p.tile_rows) * (D + 4);
+#pragma unroll
+                for (int d = 0; d < DT; d++) *(f4 *)(at + 16 * d + 4 * c) = o[x][d];
+                if (c == 0) {
+                    at[D] = m[x];
+                    at[D + 1] = l[x];
+                }
+            }
         }
+    }
+};
+
+// Where a block stands: its chunk of keys of one K/V head of one request.
+struct TreeBlock {
+    TreeReq rq;
+    int r, split, kvh, tile, group, total, t0, first, last;
+    bool whole;
+    // false: nothing to do (or done: rows of a bad request)
+    template <typename T, int D>
+    __device__ __forceinline__ bool find(const TreeP &p) {
+        split = blockIdx.x;
+        kvh = blockIdx.y % p.kv_heads;
+        tile = blockIdx.y / p.kv_heads;
+        r = blockIdx.z;
+        rq = tree_req(p, r);
+        group = p.heads / p.kv_heads;
+        whole = p.splits == 1;
+        if (rq.bad) { // may have more rows than there are tiles; the join writes them where there is one
+            if (whole && tile == 0)
+                for (int64_t e = threadIdx.x; e < (int64_t)rq.n * group * D; e += 256) {
+                    const int64_t i = e / D / group, h = kvh * group + e / D % group;
+                    ((T *)p.out)[(rq.row0 + i) * p.out_row + h * p.out_head + e % D] = fw_cvt<T>(__builtin_nanf(""));
+                }
+            return false;
+        }
+        total = rq.n * group;
+        t0 = tile * p.tile_rows;
+        if (t0 >= total) return false;
+        // a chain's rows see no further than the tile's last token
+        const int end = p.words ? rq.len + rq.n : rq.len + (min(t0 + p.tile_rows, total) - 1) / group + 1;
+        first = split * p.chunk;
+        last = min(end, first + p.chunk);
+        return whole || first < end; // the join reads no part behind the end
+    }
+};
+
+// The K or V row of key j (behind its page lookup id): address, or null where the table names no page.
+template <typename T>
+__device__ __forceinline__ const char *tree_key(const TreeP &p, const void *cache, int kvh, int j, int32_t id) {
+    const uint32_t pi = fw_div((uint32_t)j, p.page);
+    return (const char *)((const T *)cache + (int64_t)id * p.page_stride + (int64_t)(j - (int)(pi * p.page.d)) * p.token_stride +
+                          (int64_t)kvh * p.head_stride);
+}
+
+// Few rows (at most 16): the four waves take the chunk's steps of KEYS keys in
+// turn, all with the same rows, and are joined at the end.  Bound by the cache's
+// bytes, so nothing stands between memory and the lanes: a wave's K tile goes
+// straight to the registers that multiply it, its V tile through LDS of its
+// own, where the transposing read gives each lane the keys of one feature.  The
+// next step's tiles are in flight while a step computes; no barriers.
+template <typename T, int D>
+__global__ void __launch_bounds__(256, 2) k_tree_few(TreeP p) {
+    typedef Rows<T, D, 1> R;
+    constexpr int KT = R::KT, KEYS = R::KEYS, NS = R::NS;
+    constexpr int VROW = D * (int)sizeof(T) + 32; // bytes of a V row in LDS: rows 8 banks apart
+    constexpr int VBYTES = 4 * KEYS * VROW, OBYTES = 16 * D * 4;
+    __shared__ __attribute__((aligned(16))) char lds[VBYTES > OBYTES ? VBYTES : OBYTES];
+    __shared__ float sm[64], sl[64];
+    TreeBlock b;
+    if (!b.find<T, D>(p)) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4;
+    R rows;
+    rows.load(p, b.rq, b.t0, b.total, b.kvh, b.group);
+    const float zs = p.scale * 1.44269504088896340736f; // scores in base 2
+    char *vt = lds + wave * KEYS * VROW;
+    const int32_t *trow = p.table + (int64_t)b.r * p.table_stride;
+    const int last = b.last;
+
+    auto pass = [&](auto careful) {
+        constexpr bool CAREFUL = decltype(careful)::value;
+        int32_t id[KT];
+        u4 kf[KT][NS], vf[KT][NS];
+        bool gone[KT]; // no such key
+        auto pages = [&](int j) {
+#pragma unroll
+            for (int k = 0; k < KT; k++) {
+                const int key = j + k * 16 + lr;
+                id[k] = key < last ? trow[fw_div((uint32_t)key, p.page)] : -1;
+            }
+        };
+        auto load = [&](int j) {
+#pragma unroll
+            for (int k = 0; k < KT; k++) {
+                gone[k] = (uint32_t)id[k] >= (uint32_t)p.n_pages;
+                const int key = gone[k] ? 0 : j + k * 16 + lr;
+                const char *ka = tree_key<T>(p, p.kc, b.kvh, key, gone[k] ? 0 : id[k]) + c * 16;
+                const char *va = tree_key<T>(p, p.vc, b.kvh, key, gone[k] ? 0 : id[k]) + c * 16;
+#pragma unroll
+                for (int s = 0; s < NS; s++) kf[k][s] = *(const u4 *)(ka + s * 64);
+#pragma unroll
+                for (int s = 0; s < NS; s++) vf[k][s] = *(const u4 *)(va + s * 64);
+            }
+        };
+        rows.clear();
+        int j0 = b.first + wave * KEYS;
+        if (j0 < last) {
+            pages(j0);
+            load(j0);
+            pages(j0 + 4 * KEYS);
+        }
+        for (; j0 < last; j0 += 4 * KEYS) {
+            if (__any(gone[0] || gone[KT - 1])) {
+#pragma unroll
+                for (int k = 0; k < KT; k++)
+                    if (gone[k])
+#pragma unroll
+                        for (int s = 0; s < NS; s++) {
+                            kf[k][s] = ~u4{}; // NaN for whoever sees it
+                            vf[k][s] = u4{};
+                        }
+            }
+            f4 z[1][KT];
+#pragma unroll
+            for (int k = 0; k < KT; k++) {
+                f4 a = {};
+#pragma unroll
+                for (int s = 0; s < NS; s++) a = Mma<T>::dot(kf[k][s], rows.q[0][s], a);
+                z[0][k] = a * zs;
+            }
+            wave_fence();
+#pragma unroll
+            for (int k = 0; k < KT; k++)
+#pragma unroll
+                for (int s = 0; s < NS; s++)
+                    *(u4 *)(vt + (k * 16 + lr) * VROW + s * 64 + c * 16) = CAREFUL ? drop_nonfinite<T>(vf[k][s]) : vf[k][s];
+            wave_fence();
+            if (j0 + 4 * KEYS < last) {
+                load(j0 + 4 * KEYS);
+                pages(j0 + 8 * KEYS);
+            }
+            uint32_t sees[1] = {0xffffffffu};
+            if (j0 + KEYS > min(b.rq.len, last)) sees[0] = rows.mask(p, b.rq, 0, j0, last, z[0]);
+            rows.weigh(0, z[0]);
+            rows.template add<VROW>(vt, z);
+            if constexpr (CAREFUL) rows.add_dropped(p, trow, b.kvh, j0, last, z, sees);
+        }
+    };
+    pass(std::false_type{});
+    // Outputs that are not finite may come from values a row does not see (0
+    // times infinity) or from the halves of a weight (infinity less infinity):
+    // then once more, such values row by row.
+    if (__any(rows.odd())) pass(std::true_type{});
+    rows.l[0] = quarters_sum(rows.l[0]);
+    __syncthreads(); // the V tiles become the outputs' place
+    rows.join(wave, 4, 0, 16, sm, sl, (float *)lds);
+    if (wave == 0) rows.store(p, b.rq, b.r, b.tile, b.split, b.kvh, b.t0, b.total, b.whole);
+}
+
+// More rows: WR waves take RT tiles of rows each, 4 / WR waves the same rows
+// with different keys.  All share the K and V tiles of a step, which come
+// through registers into one of two places in LDS: while a step computes, the
+// next step's tiles are on their way from memory and one barrier a step
+// separates the two places.
+template <typename T, int D, int RT, int WR>
+__global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
+    typedef Rows<T, D, RT> R;
+    constexpr int KT = R::KT, KEYS = R::KEYS, NS = R::NS, WK = 4 / WR, TK = WK * KEYS; // keys of a step
+    constexpr int NC = D * (int)sizeof(T) / 16, NL = TK * NC / 256; // 16-byte pieces of a key; of a thread, for K and for V
+    constexpr int KROW = D * (int)sizeof(T) + 16;                              // rows 4 banks apart: 16-byte reads
+    constexpr int VROW = D * (int)sizeof(T) + (sizeof(T) == 2 ? 32 : 16);      // 8 apart: the transposing reads
+    constexpr int TILE = TK * (KROW + VROW), OBYTES = WK > 1 ? WR * RT * 16 * D * 4 : 0;
+    __shared__ __attribute__((aligned(16))) char lds[2 * TILE > OBYTES ? 2 * TILE : OBYTES];
+    __shared__ float sm[WK * WR * RT * 16], sl[WK * WR * RT * 16];
+    TreeBlock b;
+    if (!b.find<T, D>(p)) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4;
+    const int wr = wave / WK, wk = wave % WK, t0 = b.t0 + wr * RT * 16;
+    R rows;
+    rows.load(p, b.rq, t0, b.total, b.kvh, b.group);
+    const float zs = p.scale * 1.44269504088896340736f; // scores in base 2
+    const int32_t *trow = p.table + (int64_t)b.r * p.table_stride;
+    const int last = b.last;
+
+    auto pass = [&](auto careful) {
+        constexpr bool CAREFUL = decltype(careful)::value;
+        int32_t id[NL];
+        u4 kf[NL], vf[NL];
+        const int piece = threadIdx.x % NC, own = threadIdx.x / NC; // keys own + i * (256 / NC) of a step
+        auto pages = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int key = j + own + i * (256 / NC);
+                id[i] = key < last ? trow[fw_div((uint32_t)key, p.page)] : -1;
+            }
+        };
+        auto load = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const bool gone = (uint32_t)id[i] >= (uint32_t)p.n_pages;
+                const int key = gone ? 0 : j + own + i * (256 / NC);
+                kf[i] = *(const u4 *)(tree_key<T>(p, p.kc, b.kvh, key, gone ? 0 : id[i]) + piece * 16);
+                vf[i] = *(const u4 *)(tree_key<T>(p, p.vc, b.kvh, key, gone ? 0 : id[i]) + piece * 16);
+                if (gone) {
+                    kf[i] = ~u4{}; // NaN for whoever sees it
+                    vf[i] = u4{};
+                }
+            }
+        };
+        auto put = [&](char *at) {
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int key = own + i * (256 / NC);
+                *(u4 *)(at + key * KROW + piece * 16) = kf[i];
+                *(u4 *)(at + TK * KROW + key * VROW + piece * 16) = CAREFUL ? drop_nonfinite<T>(vf[i]) : vf[i];
+            }
+        };
+        rows.clear();
+        int j0 = b.first;
+        pages(j0);
+        load(j0);
+        pages(j0 + TK);
+        put(lds);
+        load(j0 + TK);
+        pages(j0 + 2 * TK);
         __syncthreads();
-    }
-    if (wave) return;
-    // wave 0 holds the sums
+        for (int at = 0; j0 < last; j0 += TK, at ^= 1) {
+            const char *kt = lds + at * TILE + wk * KEYS * KROW, *vt = lds + at * TILE + TK * KROW + wk * KEYS * VROW;
+            put(lds + (at ^ 1) * TILE);
+            load(j0 + 2 * TK);
+            pages(j0 + 3 * TK);
+            f4 z[RT][KT];
 #pragma unroll
-    for (int x = 0; x < RT; x++) {
-        const int t = t0 + x * 16 + lr;
-        if (t >= total) continue;
-        if (whole) {
-            T *out = (T *)p.out + (int64_t)(rq.row0 + node[x]) * p.out_row + qat[x] * p.out_head + 4 * c;
-            const bool any = tree_sees_any(p, rq, node[x]);
-            const float inv = 1.0f / l[x]; // l = 0: 0 / 0 below
+            for (int k = 0; k < KT; k++) {
+                u4 f[NS];
 #pragma unroll
-            for (int d = 0; d < DT; d++) {
-                f4 v = l[x] == 0.0f ? f4{} + __builtin_nanf("") : o[x][d] * inv;
-                if (!any) v = f4{};
-                *(typename Vec4<T>::type *)(out + 16 * d) = pack4<T>(v);
+                for (int s = 0; s < NS; s++) f[s] = *(const u4 *)(kt + (k * 16 + lr) * KROW + s * 64 + c * 16);
+#pragma unroll
+                for (int x = 0; x < RT; x++) {
+                    f4 a = {};
+#pragma unroll
+                    for (int s = 0; s < NS; s++) a = Mma<T>::dot(f[s], rows.q[x][s], a);
+                    z[x][k] = a * zs;
+                }
             }
-        } else {
-            const int64_t slot = (((int64_t)r * p.tiles + tile) * p.kv_heads + kvh) * p.splits + split;
-            float *at = p.parts + (slot * (RT * 16) + x * 16 + lr) * (D + 4);
+            const int j = j0 + wk * KEYS;
+            uint32_t sees[RT];
 #pragma unroll
-            for (int d = 0; d < DT; d++) *(f4 *)(at + 16 * d + 4 * c) = o[x][d];
-            if (c == 0) {
-                at[D] = m[x];
-                at[D + 1] = l[x];
+            for (int x = 0; x < RT; x++) {
+                sees[x] = 0xffffffffu;
+                if (j + KEYS > min(b.rq.len, last)) sees[x] = rows.mask(p, b.rq, x, j, last, z[x]);
+                rows.weigh(x, z[x]);
             }
+            rows.template add<VROW>(vt, z);
+            if constexpr (CAREFUL) rows.add_dropped(p, trow, b.kvh, j, last, z, sees);
+            __syncthreads();
         }
-    }
+    };
+    pass(std::false_type{});
+    if (__syncthreads_or(rows.odd())) pass(std::true_type{}); // as in k_tree_few
+#pragma unroll
+    for (int x = 0; x < RT; x++) rows.l[x] = quarters_sum(rows.l[x]);
+    if constexpr (WK > 1) rows.join(wk, WK, wr * RT * 16, WR * RT * 16, sm, sl, (float *)lds);
+    if (wk == 0) rows.store(p, b.rq, b.r, b.tile, b.split, b.kvh, t0, b.total, b.whole);
 }
 
 // The parts of a request's chunks into its outputs: a wave per row and head.
@@ -526,23 +665,23 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeP p) {
     }
 }
 
-// How a call of these sizes is cut.  Blocks of 16, 32 or 64 rows, so that the
-// rows of a small tree fill their tiles (f32 rows take twice the registers: 32
-// at most); the keys are split until TREE_BLOCKS blocks are there, but not into
-// chunks below TREE_CHUNK keys.
-#define TREE_BLOCKS 768
+// How a call of these sizes is cut.  Up to 16 rows per K/V head share one tile
+// (k_tree_few); 32, 64 or 128 rows a block above that (k_tree_wide).  The keys
+// are split until TREE_BLOCKS blocks are there, but not into chunks below
+// TREE_CHUNK keys.
+#define TREE_BLOCKS 1024
 #define TREE_CHUNK 256
 struct TreeCut {
-    int rt, splits, chunk;
+    int rows, splits, chunk;
     int64_t tiles;
     uint64_t bytes;
 };
 static TreeCut tree_cut(int32_t n_req, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_new,
-                        int32_t max_len, bool f32) {
+                        int32_t max_len) {
     TreeCut t;
     const int64_t rows = (int64_t)max_new * (n_heads / n_kv_heads);
-    t.rt = rows <= 16 ? 1 : rows <= 32 || f32 ? 2 : 4;
-    t.tiles = (rows + 16 * t.rt - 1) / (16 * t.rt);
+    t.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    t.tiles = (rows + t.rows - 1) / t.rows;
     const int64_t base = std::max<int64_t>(1, (int64_t)n_req * n_kv_heads * t.tiles);
     const int64_t most = std::max<int64_t>(1, ((int64_t)max_len + TREE_CHUNK - 1) / TREE_CHUNK);
     const int64_t want = std::max<int64_t>(1, std::min(most, TREE_BLOCKS / base));
@@ -550,27 +689,25 @@ static TreeCut tree_cut(int32_t n_req, int32_t n_heads, int32_t n_kv_heads, int3
     t.chunk = std::max(t.chunk, 128);
     t.splits = (int)std::max<int64_t>(1, ((int64_t)max_len + t.chunk - 1) / t.chunk);
     // enough for every smaller call too
-    t.bytes = most > 1 ? (uint64_t)std::min<int64_t>(TREE_BLOCKS, base * most) * (16 * t.rt) * (head_dim + 4) * 4 : 0;
+    t.bytes = most > 1 ? (uint64_t)std::min<int64_t>(TREE_BLOCKS, base * most) * t.rows * (head_dim + 4) * 4 : 0;
     return t;
 }
 
-template <typename T, int D, int RT>
+template <typename T, int D>
 static void tree_go(hipStream_t st, const TreeP &p, int n_req) {
-    hipLaunchKernelGGL((k_tree_attn<T, D, RT>), dim3(p.splits, p.kv_heads * p.tiles, n_req), dim3(256), 0, st, p);
+    const dim3 grid(p.splits, p.kv_heads * p.tiles, n_req), block(256);
+    if (p.tile_rows == 16) hipLaunchKernelGGL((k_tree_few<T, D>), grid, block, 0, st, p);
+    else if (p.tile_rows == 32) hipLaunchKernelGGL((k_tree_wide<T, D, 1, 2>), grid, block, 0, st, p);
+    else if (p.tile_rows == 64) hipLaunchKernelGGL((k_tree_wide<T, D, 1, 4>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((k_tree_wide<T, D, 2, 4>), grid, block, 0, st, p);
     if (p.splits > 1)
         hipLaunchKernelGGL((k_tree_join<T, D>), dim3((unsigned)((std::min(p.max_new, 4096) + 3) / 4), p.heads, n_req),
                            dim3(256), 0, st, p);
 }
-template <typename T, int D>
-static void tree_rows(hipStream_t st, const TreeP &p, int n_req, int rt) {
-    if (rt == 1) tree_go<T, D, 1>(st, p, n_req);
-    else if (rt == 2) tree_go<T, D, 2>(st, p, n_req);
-    else if constexpr (sizeof(T) == 2) tree_go<T, D, 4>(st, p, n_req);
-}
 template <typename T>
-static void tree_dim(hipStream_t st, int d, const TreeP &p, int n_req, int rt) {
-    if (d == 64) tree_rows<T, 64>(st, p, n_req, rt);
-    else tree_rows<T, 128>(st, p, n_req, rt);
+static void tree_dim(hipStream_t st, int d, const TreeP &p, int n_req) {
+    if (d == 64) tree_go<T, 64>(st, p, n_req);
+    else tree_go<T, 128>(st, p, n_req);
 }
 
 extern "C" fwhip_status fwhip_tree_attn_workspace(int32_t n_req, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
@@ -580,9 +717,7 @@ extern "C" fwhip_status fwhip_tree_attn_workspace(int32_t n_req, int32_t n_heads
         return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn_workspace: bad size");
     if (head_dim != 64 && head_dim != 128)
         return fw_fail(FWHIP_ERR_UNSUPPORTED, "fwhip_tree_attn_workspace: head_dim must be 64 or 128");
-    // the type is not asked for: whichever cut needs more
-    *bytes = std::max(tree_cut(n_req, n_heads, n_kv_heads, head_dim, max_new, max_len, false).bytes,
-                      tree_cut(n_req, n_heads, n_kv_heads, head_dim, max_new, max_len, true).bytes);
+    *bytes = tree_cut(n_req, n_heads, n_kv_heads, head_dim, max_new, max_len).bytes;
     return FWHIP_OK;
 }
 
@@ -656,17 +791,16 @@ extern "C" fwhip_status fwhip_tree_attn(fwhip_ctx *c, const fwhip_tree_attn_args
     p.row_start = a->row_start;
     p.mask = a->mask;
     p.out = a->out;
-    const TreeCut cut = tree_cut(a->n_req, a->n_heads, a->n_kv_heads, a->head_dim, std::min(a->max_new, a->n_rows), a->max_len,
-                                 a->dtype == FWHIP_T_F32);
+    const TreeCut cut = tree_cut(a->n_req, a->n_heads, a->n_kv_heads, a->head_dim, std::min(a->max_new, a->n_rows), a->max_len);
     if (cut.tiles * a->n_kv_heads > 65535)
         return fw_fail(FWHIP_ERR_UNSUPPORTED, "fwhip_tree_attn: more than 65535 row tiles x K/V heads");
     p.tiles = (int)cut.tiles;
     p.splits = cut.splits;
     p.chunk = cut.chunk;
-    p.tile_rows = 16 * cut.rt;
+    p.tile_rows = cut.rows;
     p.parts = (float *)a->workspace;
-    if (a->dtype == FWHIP_T_F32) tree_dim<float>(c->stream, a->head_dim, p, a->n_req, cut.rt);
-    else if (a->dtype == FWHIP_T_F16) tree_dim<fw_f16>(c->stream, a->head_dim, p, a->n_req, cut.rt);
-    else tree_dim<fw_bf16>(c->stream, a->head_dim, p, a->n_req, cut.rt);
+    if (a->dtype == FWHIP_T_F32) tree_dim<float>(c->stream, a->head_dim, p, a->n_req);
+    else if (a->dtype == FWHIP_T_F16) tree_dim<fw_f16>(c->stream, a->head_dim, p, a->n_req);
+    else tree_dim<fw_bf16>(c->stream, a->head_dim, p, a->n_req);
     return fw_launched("fwhip_tree_attn");
 }
