@@ -12,11 +12,16 @@
 #include "fw_paged.h"
 #include "fw_serve.h"
 
+#define TREE_BLOCKS 1024
+#define TREE_CHUNK 512
+#define TREE_ENOUGH 256
+
 struct TreeP {
     int n_req, n_rows, heads, kv_heads, n_pages, width, max_new, max_len, words;
     float scale;
     FwDiv page;
-    int64_t table_stride, q_row, q_head, out_row, out_head, page_stride, token_stride, head_stride;
+    int64_t table_stride, q_row, q_head, out_row, out_head, head_stride;
+    uint32_t page_bytes, token_bytes;
     const void *q, *kc, *vc;
     const int32_t *table, *len, *row_start;
     const uint64_t *mask;
@@ -52,7 +57,7 @@ struct Mma<fw_f16> {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const auto h = __builtin_amdgcn_cvt_pkrtz(p[2 * i], p[2 * i + 1]);
-            const auto l = __builtin_amdgcn_cvt_pkrtz(p[2 * i] - (float)h[0], p[2 * i + 1] - (float)h[1]);
+            const auto l = __builtin_amdgcn_cvt_pkrtz(fmaf((float)h[0], -1.0f, p[2 * i]), fmaf((float)h[1], -1.0f, p[2 * i + 1]));
             hi[i] = __builtin_bit_cast(uint32_t, h);
             lo[i] = __builtin_bit_cast(uint32_t, l);
         }
@@ -166,6 +171,33 @@ __device__ __forceinline__ typename Vec4<T>::type pack4(f4 v) {
                           fw_cvt<T>(v[2]).b | (uint32_t)fw_cvt<T>(v[3]).b << 16);
 }
 
+// Bytes from the start of a K/V head's cache to key j of the request, whose page is id.
+__device__ __forceinline__ uint64_t tree_at(const TreeP &p, uint32_t j, uint32_t id) {
+    const uint32_t t = j - fw_div(j, p.page) * p.page.d;
+    return (uint64_t)id * p.page_bytes + (uint64_t)t * p.token_bytes;
+}
+
+// Scores are z = zs * (q . k) with zs > 0 in base 2, so that the largest product
+// has the largest score: a negative scale turns q's signs, a scale of zero
+// makes q zero (NaN where it is not finite).
+__device__ __forceinline__ float tree_zs(const TreeP &p) {
+    return p.scale == 0.0f ? 1.0f : fabsf(p.scale) * 1.44269504088896340736f;
+}
+template <typename T>
+__device__ __forceinline__ u4 tree_query(u4 v, float scale) {
+    if (scale > 0.0f) return v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (scale < 0.0f) v[i] ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+        else if constexpr (sizeof(T) == 4) v[i] = (v[i] & 0x7f800000u) == 0x7f800000u ? 0x7fc00000u : 0;
+        else {
+            constexpr uint32_t E = std::is_same<T, fw_f16>::value ? 0x7c00u : 0x7f80u;
+            v[i] = ((v[i] & E) == E ? 0x7fffu : 0) | ((v[i] >> 16 & E) == E ? 0x7fff0000u : 0);
+        }
+    }
+    return v;
+}
+
 // ---------------------------------------------------------------------------
 // What both kernels below do with a wave's rows: RT tiles of 16 query rows (new
 // token x query head of the K/V head's group), and steps of KEYS keys.
@@ -186,7 +218,7 @@ struct Rows {
             head[x] = kvh * group + t % group;
             const T *at = (const T *)p.q + (int64_t)(rq.row0 + node[x]) * p.q_row + head[x] * p.q_head;
 #pragma unroll
-            for (int s = 0; s < NS; s++) q[x][s] = *(const u4 *)((const char *)at + s * 64 + c * 16);
+            for (int s = 0; s < NS; s++) q[x][s] = tree_query<T>(*(const u4 *)((const char *)at + s * 64 + c * 16), p.scale);
         }
     }
     __device__ __forceinline__ void clear() {
@@ -198,7 +230,7 @@ struct Rows {
             for (int d = 0; d < DT; d++) o[x][d] = f4{};
         }
     }
-    // Scores of the step at key j to -inf where a row does not see the key; the
+    // Products of the step at key j to -inf where a row does not see the key; the
     // keys it sees as bits (4 per key tile).
     __device__ __forceinline__ uint32_t mask(const TreeP &p, const TreeReq &rq, int x, int j, int last, f4 (&z)[KT]) const {
         const int c = (threadIdx.x & 63) >> 4;
@@ -216,14 +248,14 @@ struct Rows {
             }
         return sees;
     }
-    // Scores to weights (in place); what is there already is scaled to the new maximum.
-    __device__ __forceinline__ void weigh(int x, f4 (&z)[KT]) {
+    // Products q . k to weights (in place); what is there already is scaled to the new maximum.
+    __device__ __forceinline__ void weigh(int x, f4 (&z)[KT], float zs) {
         float mx = z[0][0];
 #pragma unroll
         for (int k = 0; k < KT; k++)
 #pragma unroll
             for (int i = 0; i < 4; i++) mx = fmaxf(mx, z[k][i]);
-        mx = quarters_max(mx);
+        mx = quarters_max(mx) * zs;
         if (__any(mx > m[x])) {
             const float mn = fmaxf(mx, m[x]), f = __builtin_amdgcn_exp2f(m[x] - TREE_BIAS - tree_base(mn));
             m[x] = mn;
@@ -236,7 +268,8 @@ struct Rows {
         for (int k = 0; k < KT; k++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                z[k][i] = __builtin_amdgcn_exp2f(z[k][i] - base);
+                // rounded before the difference, as the maximum is: its own weight is exact at any size
+                z[k][i] = __builtin_amdgcn_exp2f(z[k][i] * zs - base);
                 l[x] += z[k][i];
             }
     }
@@ -280,11 +313,9 @@ struct Rows {
         const int lane = threadIdx.x & 63, lr = lane & 15, c = lane >> 4;
         for (int key = 0; key < KEYS && j + key < last; key++) {
             const int from = ((key & 15) >> 2) * 16 + lr, slot = (key >> 4) * 4 + (key & 3);
-            const uint32_t pi = fw_div((uint32_t)(j + key), p.page);
-            const int32_t id = trow[pi];
+            const int32_t id = trow[fw_div((uint32_t)(j + key), p.page)];
             if ((uint32_t)id >= (uint32_t)p.n_pages) continue;
-            const T *v = (const T *)p.vc + id * p.page_stride + (int64_t)(j + key - pi * p.page.d) * p.token_stride +
-                         kvh * p.head_stride;
+            const T *v = (const T *)((const char *)((const T *)p.vc + kvh * p.head_stride) + tree_at(p, j + key, id));
 #pragma unroll
             for (int x = 0; x < RT; x++) {
                 float mine = 0.0f;
@@ -417,14 +448,6 @@ struct TreeBlock {
     }
 };
 
-// The K or V row of key j (behind its page lookup id): address, or null where the table names no page.
-template <typename T>
-__device__ __forceinline__ const char *tree_key(const TreeP &p, const void *cache, int kvh, int j, int32_t id) {
-    const uint32_t pi = fw_div((uint32_t)j, p.page);
-    return (const char *)((const T *)cache + (int64_t)id * p.page_stride + (int64_t)(j - (int)(pi * p.page.d)) * p.token_stride +
-                          (int64_t)kvh * p.head_stride);
-}
-
 // Few rows (at most 16): the four waves take the chunk's steps of KEYS keys in
 // turn, all with the same rows, and are joined at the end.  Bound by the cache's
 // bytes, so nothing stands between memory and the lanes: a wave's K tile goes
@@ -444,9 +467,11 @@ __global__ void __launch_bounds__(256, 2) k_tree_few(TreeP p) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4;
     R rows;
     rows.load(p, b.rq, b.t0, b.total, b.kvh, b.group);
-    const float zs = p.scale * 1.44269504088896340736f; // scores in base 2
+    const float zs = tree_zs(p);
     char *vt = lds + wave * KEYS * VROW;
     const int32_t *trow = p.table + (int64_t)b.r * p.table_stride;
+    const char *kbase = (const char *)((const T *)p.kc + b.kvh * p.head_stride) + c * 16;
+    const char *vbase = (const char *)((const T *)p.vc + b.kvh * p.head_stride) + c * 16;
     const int last = b.last;
 
     auto pass = [&](auto careful) {
@@ -465,9 +490,8 @@ __global__ void __launch_bounds__(256, 2) k_tree_few(TreeP p) {
 #pragma unroll
             for (int k = 0; k < KT; k++) {
                 gone[k] = (uint32_t)id[k] >= (uint32_t)p.n_pages;
-                const int key = gone[k] ? 0 : j + k * 16 + lr;
-                const char *ka = tree_key<T>(p, p.kc, b.kvh, key, gone[k] ? 0 : id[k]) + c * 16;
-                const char *va = tree_key<T>(p, p.vc, b.kvh, key, gone[k] ? 0 : id[k]) + c * 16;
+                const uint64_t at = gone[k] ? 0 : tree_at(p, j + k * 16 + lr, id[k]);
+                const char *ka = kbase + at, *va = vbase + at;
 #pragma unroll
                 for (int s = 0; s < NS; s++) kf[k][s] = *(const u4 *)(ka + s * 64);
 #pragma unroll
@@ -498,7 +522,7 @@ __global__ void __launch_bounds__(256, 2) k_tree_few(TreeP p) {
                 f4 a = {};
 #pragma unroll
                 for (int s = 0; s < NS; s++) a = Mma<T>::dot(kf[k][s], rows.q[0][s], a);
-                z[0][k] = a * zs;
+                z[0][k] = a;
             }
             wave_fence();
 #pragma unroll
@@ -513,7 +537,7 @@ __global__ void __launch_bounds__(256, 2) k_tree_few(TreeP p) {
             }
             uint32_t sees[1] = {0xffffffffu};
             if (j0 + KEYS > min(b.rq.len, last)) sees[0] = rows.mask(p, b.rq, 0, j0, last, z[0]);
-            rows.weigh(0, z[0]);
+            rows.weigh(0, z[0], zs);
             rows.template add<VROW>(vt, z);
             if constexpr (CAREFUL) rows.add_dropped(p, trow, b.kvh, j0, last, z, sees);
         }
@@ -550,15 +574,18 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
     const int wr = wave / WK, wk = wave % WK, t0 = b.t0 + wr * RT * 16;
     R rows;
     rows.load(p, b.rq, t0, b.total, b.kvh, b.group);
-    const float zs = p.scale * 1.44269504088896340736f; // scores in base 2
+    const float zs = tree_zs(p);
     const int32_t *trow = p.table + (int64_t)b.r * p.table_stride;
+    const int piece = threadIdx.x % NC, own = threadIdx.x / NC; // keys own + i * (256 / NC) of a step
+    const char *kbase = (const char *)((const T *)p.kc + b.kvh * p.head_stride) + piece * 16;
+    const char *vbase = (const char *)((const T *)p.vc + b.kvh * p.head_stride) + piece * 16;
     const int last = b.last;
 
     auto pass = [&](auto careful) {
         constexpr bool CAREFUL = decltype(careful)::value;
         int32_t id[NL];
         u4 kf[NL], vf[NL];
-        const int piece = threadIdx.x % NC, own = threadIdx.x / NC; // keys own + i * (256 / NC) of a step
+        bool gone[NL]; // no such key
         auto pages = [&](int j) {
 #pragma unroll
             for (int i = 0; i < NL; i++) {
@@ -569,17 +596,24 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
         auto load = [&](int j) {
 #pragma unroll
             for (int i = 0; i < NL; i++) {
-                const bool gone = (uint32_t)id[i] >= (uint32_t)p.n_pages;
-                const int key = gone ? 0 : j + own + i * (256 / NC);
-                kf[i] = *(const u4 *)(tree_key<T>(p, p.kc, b.kvh, key, gone ? 0 : id[i]) + piece * 16);
-                vf[i] = *(const u4 *)(tree_key<T>(p, p.vc, b.kvh, key, gone ? 0 : id[i]) + piece * 16);
-                if (gone) {
-                    kf[i] = ~u4{}; // NaN for whoever sees it
-                    vf[i] = u4{};
-                }
+                gone[i] = (uint32_t)id[i] >= (uint32_t)p.n_pages;
+                const uint64_t at = gone[i] ? 0 : tree_at(p, j + own + i * (256 / NC), id[i]);
+                kf[i] = *(const u4 *)(kbase + at);
+                vf[i] = *(const u4 *)(vbase + at);
             }
         };
         auto put = [&](char *at) {
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < NL; i++) any |= gone[i];
+            if (__any(any)) {
+#pragma unroll
+                for (int i = 0; i < NL; i++)
+                    if (gone[i]) {
+                        kf[i] = ~u4{}; // NaN for whoever sees it
+                        vf[i] = u4{};
+                    }
+            }
 #pragma unroll
             for (int i = 0; i < NL; i++) {
                 const int key = own + i * (256 / NC);
@@ -612,7 +646,7 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
                     f4 a = {};
 #pragma unroll
                     for (int s = 0; s < NS; s++) a = Mma<T>::dot(f[s], rows.q[x][s], a);
-                    z[x][k] = a * zs;
+                    z[x][k] = a;
                 }
             }
             const int j = j0 + wk * KEYS;
@@ -621,7 +655,7 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
             for (int x = 0; x < RT; x++) {
                 sees[x] = 0xffffffffu;
                 if (j + KEYS > min(b.rq.len, last)) sees[x] = rows.mask(p, b.rq, x, j, last, z[x]);
-                rows.weigh(x, z[x]);
+                rows.weigh(x, z[x], zs);
             }
             rows.template add<VROW>(vt, z);
             if constexpr (CAREFUL) rows.add_dropped(p, trow, b.kvh, j, last, z, sees);
@@ -636,32 +670,70 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
     if (wk == 0) rows.store(p, b.rq, b.r, b.tile, b.split, b.kvh, t0, b.total, b.whole);
 }
 
-// The parts of a request's chunks into its outputs: a wave per row and head.
-template <typename T, int D>
+// The parts of a request's chunks into its outputs: NW waves a row and head.
+// The parts' weights first (a lane each), then the sum, D / 4 lanes a part and
+// 256 NW / D parts at once.  NW = 1 holds the weights in its lanes (at most 64).
+template <typename T, int D, int NW>
 __global__ void __launch_bounds__(256) k_tree_join(TreeP p) {
-    const int lane = threadIdx.x & 63, r = blockIdx.z, h = blockIdx.y;
+    constexpr int W = D / 4, N = 64 * NW, G = N / W;
+    __shared__ float weight[NW == 1 ? 1 : TREE_BLOCKS], red[8];
+    __shared__ f4 sum[256 / W][W];
+    const int r = blockIdx.z, h = blockIdx.y, tid = threadIdx.x % N, own = threadIdx.x / N;
     const TreeReq rq = tree_req(p, r);
     const int group = p.heads / p.kv_heads, kvh = h / group;
-    for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < rq.n; i += gridDim.x * 4) {
-        const int t = i * group + h % group, tile = t / p.tile_rows;
-        const int keys = rq.bad ? 0 : p.words ? rq.len + rq.n
-            : min(rq.len + rq.n, rq.len + (min((tile + 1) * p.tile_rows, rq.n * group) - 1) / group + 1);
-        const int parts = (keys + p.chunk - 1) / p.chunk;
+    for (int64_t i = (int64_t)blockIdx.x * (256 / N) + own; i < rq.n; i += (int64_t)gridDim.x * (256 / N)) {
+        T *out = (T *)p.out + (rq.row0 + i) * p.out_row + (int64_t)h * p.out_head;
+        if (rq.bad || !tree_sees_any(p, rq, (int)i)) { // the same for the row's waves
+            const float v = rq.bad ? __builtin_nanf("") : 0.0f;
+            if (tid < W) *(typename Vec4<T>::type *)(out + 4 * tid) = pack4<T>(f4{v, v, v, v});
+            continue;
+        }
+        const int t = (int)i * group + h % group, tile = t / p.tile_rows;
+        const int keys = rq.len + (p.words ? rq.n : (min((tile + 1) * p.tile_rows, rq.n * group) - 1) / group + 1);
+        const int parts = (keys + p.chunk - 1) / p.chunk; // at most p.splits
         const int64_t slot = (((int64_t)r * p.tiles + tile) * p.kv_heads + kvh) * p.splits;
         const float *at = p.parts + (slot * p.tile_rows + t % p.tile_rows) * (D + 4);
         const int64_t step = (int64_t)p.tile_rows * (D + 4);
-        float mx = -INFINITY;
-        for (int s = 0; s < parts; s++) mx = fmaxf(mx, at[s * step + D]);
-        float l = 0.0f, o[D / 64] = {};
-        for (int s = 0; s < parts; s++) {
-            const float f = __builtin_amdgcn_exp2f(at[s * step + D] - TREE_BIAS - tree_base(mx));
-            l = fmaf(f, at[s * step + D + 1], l);
-            for (int x = 0; x < D / 64; x++) o[x] = fmaf(f, at[s * step + x * 64 + lane], o[x]);
+        float mx = -INFINITY, l = 0.0f, mine = -INFINITY;
+        if constexpr (NW == 1) {
+            if (tid < parts) mine = at[tid * step + D];
+            mx = fw_wave_max(mine);
+            mine = __builtin_amdgcn_exp2f(mine - TREE_BIAS - tree_base(mx));
+            if (tid < parts) l = mine * at[tid * step + D + 1];
+            l = fw_wave_sum(l);
+        } else {
+            __syncthreads();
+            for (int s = tid; s < parts; s += N) mx = fmaxf(mx, weight[s] = at[s * step + D]);
+            mx = fw_block_max(mx, red);
+            for (int s = tid; s < parts; s += N) {
+                const float f = __builtin_amdgcn_exp2f(weight[s] - TREE_BIAS - tree_base(mx));
+                weight[s] = f;
+                l = fmaf(f, at[s * step + D + 1], l);
+            }
+            l = fw_block_sum(l, red);
         }
-        T *out = (T *)p.out + (int64_t)(rq.row0 + i) * p.out_row + (int64_t)h * p.out_head;
-        const bool any = rq.bad || tree_sees_any(p, rq, i);
-        for (int x = 0; x < D / 64; x++)
-            out[x * 64 + lane] = fw_cvt<T>(!any ? 0.0f : l == 0.0f ? __builtin_nanf("") : o[x] / l);
+        f4 o = {};
+#pragma unroll 4
+        for (int s0 = 0; s0 < parts; s0 += G) { // the same turns for every lane: the exchange needs them all
+            const int s = s0 + tid / W;
+            const float f = NW == 1 ? __shfl(mine, s) : weight[min(s, parts - 1)];
+            if (s < parts) {
+                const f4 v = *(const f4 *)(at + s * step + 4 * (tid % W));
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] = fmaf(f, v[e], o[e]);
+            }
+        }
+        f4 *all = &sum[own * G][0];
+        all[tid] = o;
+        if constexpr (NW == 1) wave_fence();
+        else __syncthreads();
+        if (tid < W) {
+#pragma unroll
+            for (int g = 1; g < G; g++) o += all[g * W + tid];
+            const float inv = 1.0f / l;
+            *(typename Vec4<T>::type *)(out + 4 * tid) = pack4<T>(l == 0.0f ? f4{} + __builtin_nanf("") : o * inv);
+        }
+        if constexpr (NW == 1) wave_fence();
     }
 }
 
@@ -669,8 +741,6 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeP p) {
 // (k_tree_few); 32, 64 or 128 rows a block above that (k_tree_wide).  The keys
 // are split until TREE_BLOCKS blocks are there, but not into chunks below
 // TREE_CHUNK keys.
-#define TREE_BLOCKS 1024
-#define TREE_CHUNK 256
 struct TreeCut {
     int rows, splits, chunk;
     int64_t tiles;
@@ -684,7 +754,8 @@ static TreeCut tree_cut(int32_t n_req, int32_t n_heads, int32_t n_kv_heads, int3
     t.tiles = (rows + t.rows - 1) / t.rows;
     const int64_t base = std::max<int64_t>(1, (int64_t)n_req * n_kv_heads * t.tiles);
     const int64_t most = std::max<int64_t>(1, ((int64_t)max_len + TREE_CHUNK - 1) / TREE_CHUNK);
-    const int64_t want = std::max<int64_t>(1, std::min(most, TREE_BLOCKS / base));
+    const int64_t blocks = t.rows == 128 ? TREE_BLOCKS / 2 : TREE_BLOCKS;
+    const int64_t want = base >= TREE_ENOUGH ? 1 : std::max<int64_t>(1, std::min(most, blocks / base));
     t.chunk = (int)((((int64_t)max_len + want - 1) / want + 127) / 128 * 128);
     t.chunk = std::max(t.chunk, 128);
     t.splits = (int)std::max<int64_t>(1, ((int64_t)max_len + t.chunk - 1) / t.chunk);
@@ -700,9 +771,10 @@ static void tree_go(hipStream_t st, const TreeP &p, int n_req) {
     else if (p.tile_rows == 32) hipLaunchKernelGGL((k_tree_wide<T, D, 1, 2>), grid, block, 0, st, p);
     else if (p.tile_rows == 64) hipLaunchKernelGGL((k_tree_wide<T, D, 1, 4>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((k_tree_wide<T, D, 2, 4>), grid, block, 0, st, p);
-    if (p.splits > 1)
-        hipLaunchKernelGGL((k_tree_join<T, D>), dim3((unsigned)((std::min(p.max_new, 4096) + 3) / 4), p.heads, n_req),
-                           dim3(256), 0, st, p);
+    if (p.splits == 1) return;
+    const unsigned rows = (unsigned)std::min(p.max_new, 4096);
+    if (p.splits <= 64) hipLaunchKernelGGL((k_tree_join<T, D, 1>), dim3((rows + 3) / 4, p.heads, n_req), block, 0, st, p);
+    else hipLaunchKernelGGL((k_tree_join<T, D, 4>), dim3(rows, p.heads, n_req), block, 0, st, p);
 }
 template <typename T>
 static void tree_dim(hipStream_t st, int d, const TreeP &p, int n_req) {
@@ -751,6 +823,9 @@ extern "C" fwhip_status fwhip_tree_attn(fwhip_ctx *c, const fwhip_tree_attn_args
                 return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn: strides must be multiples of 16 bytes");
         if (a->out == a->q) return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn: out must not be q");
     }
+    if (a->page_stride > 0x3fffffff || a->token_stride > 0x3fffffff)
+        return fw_fail(FWHIP_ERR_UNSUPPORTED, "fwhip_tree_attn: page and token strides must be below 2^30 elements");
+    if (!(fabsf(a->scale) < INFINITY)) return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn: scale must be finite");
     if (a->mask ? a->mask_words < 1 || (int64_t)a->mask_words * 64 < a->max_new : a->mask_words != 0)
         return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn: mask needs 64 * mask_words >= max_new (mask_words 0 without)");
     uint64_t need = 0;
@@ -780,8 +855,8 @@ extern "C" fwhip_status fwhip_tree_attn(fwhip_ctx *c, const fwhip_tree_attn_args
     p.q_head = a->q_head;
     p.out_row = a->out_row;
     p.out_head = a->out_head;
-    p.page_stride = a->page_stride;
-    p.token_stride = a->token_stride;
+    p.page_bytes = (uint32_t)(a->page_stride * fw_dtype_bytes(a->dtype));
+    p.token_bytes = (uint32_t)(a->token_stride * fw_dtype_bytes(a->dtype));
     p.head_stride = a->head_stride;
     p.q = a->q;
     p.kc = a->k_cache;

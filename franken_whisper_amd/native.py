@@ -176,6 +176,7 @@ class Context:
         else:
             check(lib().fwhip_init_on_stream(device, stream, C.byref(h)))
         self.h = h
+        self.device = device
 
     def array(self, a: np.ndarray) -> DeviceArray:
         return DeviceArray(self, a.shape, a.dtype).upload(a)

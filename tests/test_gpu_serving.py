@@ -380,6 +380,16 @@ def test_attention_infinite_scores(tctx, kind):
     check_attn(tctx, s)
 
 
+@pytest.mark.parametrize("kind", DT)
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-3, 2.0])
+def test_attention_scales(tctx, kind, scale):
+    """Negative scales, zero (the mean of what a row sees) and sharp ones."""
+    for n_new, heads in (([5, 9], 2), ([30, 60], 4)):
+        s = attn_inputs(30, kind, [77, 300], n_new, heads, 2, 64, 16, True, empty=0.2)
+        s["scale"] = scale
+        check_attn(tctx, s)
+
+
 def test_attention_bad_requests_come_out_as_nan(tctx):
     s = attn_inputs(12, "f16", [40, 50, 60, 70, 20], [3, 4, 5, 2, 1], 4, 2, 64, 16, True)
     want, tol = reference(s)

@@ -87,7 +87,7 @@ def test_append_refusals(kw, word):
     (dict(max_new=-1), "negative size"), (dict(max_len=-1), "negative size"), (dict(n_pages=-1), "negative size"),
     (dict(n_heads=7), "n_kv_heads"), (dict(n_kv_heads=0), "n_kv_heads"), (dict(n_heads=0), "n_kv_heads"),
     (dict(page_size=0), "page_size"), (dict(max_len=129), "max_len"), (dict(n_req=65536), "n_req"),
-    (dict(q_row=-8), "negative stride"), (dict(table_stride=-1), "negative stride"), (dict(q=None), "NULL"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(q_row=-8), "negative stride"), (dict(table_stride=-1), "negative stride"), (dict(q=None), "NULL"),
     (dict(table=None), "NULL"), (dict(row_start=None), "NULL"), (dict(len=None), "NULL"), (dict(out=None), "NULL"),
     (dict(k_cache=None), "NULL"), (dict(q=A + 8), "16-byte"), (dict(v_cache=3 * A + 4), "16-byte"),
     (dict(q_head=4), "multiples of 16"), (dict(page_stride=2047), "multiples of 16"), (dict(out=A), "out must not"),
@@ -100,6 +100,11 @@ def test_attention_refusals(kw, word):
 def test_attention_head_dims_that_are_not_built():
     for d in (0, 32, 63, 80, 256):
         _says("fwhip_tree_attn", _set(_attn, head_dim=d), "head_dim", abi.ERR_UNSUPPORTED)
+
+
+def test_attention_strides_past_the_addressing():
+    _says("fwhip_tree_attn", _set(_attn, page_stride=1 << 30), "strides", abi.ERR_UNSUPPORTED)
+    _says("fwhip_tree_attn", _set(_attn, token_stride=1 << 30), "strides", abi.ERR_UNSUPPORTED)
 
 
 def test_attention_workspace_is_checked():
@@ -179,7 +184,16 @@ class _Dev:
 
 
 class _Ctx:
-    h = None
+    h, device = None, 0
+
+
+def test_python_refuses_tensors_off_the_contexts_device():
+    torch = pytest.importorskip("torch")
+    x, q, s, y = torch.zeros(2, 64), torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 2).half(), torch.zeros(2, 8)
+    with pytest.raises(ValueError, match="x must be on the context's device"):
+        ops.q4_linear(_Ctx, x, q, s, y)
+    with pytest.raises(ValueError, match="element type torch.float64"):
+        ops.q4_linear(_Ctx, x.double(), q, s, y.double())
 
 
 def test_python_checks_shapes_and_types():
