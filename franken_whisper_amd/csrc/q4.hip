@@ -18,7 +18,7 @@ struct Q4P {
     const void *scale, *minimum;
     const float *bias;
     void *y;
-    int scale32, vec, shift; // planes of f32; x rows 16-byte (f32) or 8-byte aligned; log2 of the group's blocks
+    int scale32, vec, pair; // planes of f32; x rows 16-byte (f32) or 8-byte aligned; four f16 scales so aligned
     int chunk, lds;          // inputs staged at a time; bytes of LDS
 };
 
@@ -53,33 +53,37 @@ __device__ __forceinline__ f4 q4_quarters(float v) {
 // f16: a code in the low bits of 1024 (or, four bits up, of 64) is that number
 // plus the code; what is too much is taken off again, exactly, and with it the
 // 8 of weights without minimums.
+struct Q4Magic { // in registers: an instruction that masks and sets bits takes one constant from the scalars, none from the code
+    uint32_t lo, hi;
+};
+__device__ __forceinline__ uint32_t q4_bits(uint32_t w, uint32_t mask, uint32_t set) { return (w & mask) | set; }
 template <bool MIN>
-__device__ __forceinline__ u4 q4_codes_f16(uint32_t w) {
+__device__ __forceinline__ u4 q4_codes_f16(uint32_t w, Q4Magic k) {
     const uint32_t v = w >> 8;
     const h2 lo = MIN ? h2{(_Float16)1024, (_Float16)1024} : h2{(_Float16)1032, (_Float16)1032};
     const h2 hi = MIN ? h2{(_Float16)64, (_Float16)64} : h2{(_Float16)72, (_Float16)72};
     u4 r;
-    r[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (w & 0x000f000fu) | 0x64006400u) - lo);
-    r[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (w & 0x00f000f0u) | 0x54005400u) - hi);
-    r[2] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (v & 0x000f000fu) | 0x64006400u) - lo);
-    r[3] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (v & 0x00f000f0u) | 0x54005400u) - hi);
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, q4_bits(w, 0x000f000fu, k.lo)) - lo);
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, q4_bits(w, 0x00f000f0u, k.hi)) - hi);
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, q4_bits(v, 0x000f000fu, k.lo)) - lo);
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, q4_bits(v, 0x00f000f0u, k.hi)) - hi);
     return r;
 }
 // bf16: 128 + code; there is no packed bf16 subtraction, so the 128 (and the 8)
 // leave with the sums of the inputs (CORR below).  That costs five bits of the
 // f32 sum, 2^-19 of the result against the 2^-9 of its rounding.
-__device__ __forceinline__ u4 q4_codes_bf16(uint32_t w) {
+__device__ __forceinline__ u4 q4_codes_bf16(uint32_t w, Q4Magic k) {
     u4 r;
 #pragma unroll
-    for (int i = 0; i < 4; i++) r[i] = (w >> (4 * i) & 0x000f000fu) | 0x43004300u;
+    for (int i = 0; i < 4; i++) r[i] = q4_bits(w >> (4 * i), 0x000f000fu, k.lo);
     return r;
 }
 
-// x in LDS, as the products read it: per row KC inputs of 16 bits in units of 8,
-// the unit (block, c) holding inputs 4 c + 0, 2, 16, 18, 1, 3, 17, 19 of its
+// x in LDS, as the products read it: per row `chunk` inputs of 16 bits in units
+// of 8, the unit (block, c) holding inputs 4 c + 0, 2, 16, 18, 1, 3, 17, 19 of its
 // block.  f16 and bf16 as they are; f32 as two f16 parts of x / s, where s is
-// the power of two that takes the largest |x| of the row's 128 to 2^14..2^15:
-// hi + lo is within 2^-22 of x down to 2^-28 of that largest.
+// the power of two that takes the largest |x| of the row's turn of inputs to
+// 2^14..2^15: hi + lo is within 2^-22 of x down to 2^-28 of that largest.
 template <typename T>
 struct Q4X {
     static constexpr int PARTS = std::is_same<T, float>::value ? 2 : 1;
@@ -127,78 +131,113 @@ __device__ __forceinline__ float q4_one(const Q4P &p, int m, int n) {
 }
 
 // The kernel: MT * 16 rows of x by WN waves of NT * 16 outputs each, WK waves
-// taking the steps of the same outputs in turn.  x is staged in LDS for up to
-// `chunk` inputs at a time, its block sums beside it where weights have a
-// minimum; each wave streams its weights straight to registers, U steps ahead.
-// GB = 4: one scale a step (groups of 128), else one a block.
-template <typename T, bool MIN, int GB, int MT, int NT, int WN, int WK, int U>
+// taking turns of MS steps of the same outputs.  x is staged in LDS for up to
+// `chunk` inputs at a time, its sums beside it where weights have a minimum;
+// each wave streams its weights straight to registers, one turn ahead.  GB: the
+// 32-weight blocks of a group.  Of a turn's 4 MS blocks a lane quarter loads the
+// scales of its MS, which the quarters then exchange.
+template <typename T, bool MIN, int GB, int MT, int NT, int WN, int WK, int MS>
 __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
     constexpr bool BF = std::is_same<T, fw_bf16>::value, F32 = std::is_same<T, float>::value, CORR = MIN || BF;
-    constexpr int PARTS = Q4X<T>::PARTS, NTH = 64 * WN * WK;
+    constexpr int PARTS = Q4X<T>::PARTS, NW = WN * WK, R = MT * 16;
+    constexpr int SP = MS > GB ? MS / GB : 1;     // scales a lane loads a turn
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, c = lane >> 4;
+    const int lane = threadIdx.x & 63, lr = lane & 15, c = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); // the same in all lanes: loops and branches stay scalar
     const int wn = wave / WK, wk = wave % WK;
-    const int m0 = blockIdx.y * MT * 16, rows = min(MT * 16, p.m - m0);
+    const int m0 = blockIdx.y * R, rows = min(R, p.m - m0);
     const int n0 = (blockIdx.x * WN + wn) * NT * 16;
-    const int steps = (p.k + 127) / 128, csteps = p.chunk / 128;
+    const int cturns = p.chunk / (128 * MS), turns = (p.k + 128 * MS - 1) / (128 * MS);
     const int xrow = p.chunk * 2 + 16; // bytes of a row: rows 4 banks apart
     const int plane = rows * xrow;
-    int *odd = (int *)lds;                                    // [MT * 16]: rows with a value that is not finite
-    char *xt = lds + MT * 64;                                 // x: [part][row][xrow]
-    float *sums = (float *)(xt + PARTS * plane);              // CORR: [step][block][MT * 16]
-    float *scal = sums + (CORR ? csteps * 4 * MT * 16 : 0);   // f32: [step][MT * 16]
+    int *odd = (int *)lds;                                      // [R]: rows with a value that is not finite
+    char *xt = lds + R * 4;                                     // x: [part][row][xrow]
+    float *sums = (float *)(xt + PARTS * plane);                // CORR: [turn][MS][4][R], see below
+    float *scal = sums + (CORR ? cturns * MS * 4 * R : 0);      // f32: [turn][R]
+    Q4Magic magic = BF ? Q4Magic{0x43004300u, 0} : Q4Magic{0x64006400u, 0x54005400u};
+    asm volatile("" : "+v"(magic.lo), "+v"(magic.hi));
 
-    f4 acc[MT][NT], mid[MT][NT];
+    f4 acc[MT][NT];
 #pragma unroll
     for (int x = 0; x < MT; x++)
 #pragma unroll
         for (int y = 0; y < NT; y++) acc[x][y] = f4{};
     if (CORR)
-        for (int i = threadIdx.x; i < MT * 16; i += NTH) odd[i] = 0;
+        for (int i = threadIdx.x; i < R; i += 64 * NW) odd[i] = 0;
 
-    int nrow[NT];
+    const int groups = p.k / (32 * GB), blocks = p.k / 32;
+    const uint8_t *qrow[NT];
+    int64_t srow[NT];
 #pragma unroll
-    for (int y = 0; y < NT; y++) nrow[y] = min(n0 + y * 16 + lr, p.n - 1); // the last again behind the end
-    u4 wq[U][NT];
-    float sc[U][NT], mn[U][NT];
-    const int groups = p.k / p.group;
-    auto load = [&](int s0, int to) { // steps s0, s0 + WK, ... below `to`
+    for (int y = 0; y < NT; y++) {
+        const int n = min(n0 + y * 16 + lr, p.n - 1); // the last again behind the end
+        qrow[y] = p.q + (int64_t)n * (p.k / 2);
+        srow[y] = (int64_t)n * groups;
+    }
+    // a turn's weights and scales, as stored (converting here would wait for them)
+    u4 wq[MS][NT];
+    uint32_t sc[SP][NT], mn[SP][NT];
+    auto load = [&](int t) {
+        const bool whole = (t + 1) * 4 * MS <= blocks;
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int s = s0 + u * WK, blk = s * 4 + c;
-            const bool in = s < to && blk * 32 < p.k;
-            const int g = blk >> p.shift;
+        for (int y = 0; y < NT; y++) {
 #pragma unroll
-            for (int y = 0; y < NT; y++) {
-                wq[u][y] = u4{};
-                sc[u][y] = mn[u][y] = 0.0f;
-                if (!in) continue;
-                wq[u][y] = *(const u4 *)(p.q + (int64_t)nrow[y] * (p.k / 2) + blk * 16);
-                const int64_t at = (int64_t)nrow[y] * groups + g;
-                if (p.scale32) {
-                    sc[u][y] = ((const float *)p.scale)[at];
-                    if (MIN) mn[u][y] = ((const float *)p.minimum)[at];
-                } else {
-                    sc[u][y] = fw_to_f32(((const fw_f16 *)p.scale)[at]);
-                    if (MIN) mn[u][y] = fw_to_f32(((const fw_f16 *)p.minimum)[at]);
+            for (int u = 0; u < MS; u++) {
+                int blk = (t * MS + u) * 4 + c;
+                if (!whole) blk = min(blk, blocks - 1);
+                wq[u][y] = *(const u4 *)(qrow[y] + (uint32_t)blk * 16);
+            }
+            const int g = (t * 4 + c) * MS / GB; // the first of this quarter's groups
+            if (!p.scale32 && p.pair && SP == 4 && whole) { // four f16 in one load
+                const uint2 a = *(const uint2 *)((const uint16_t *)p.scale + srow[y] + g);
+                sc[0][y] = a.x, sc[1][y] = a.x >> 16, sc[2][y] = a.y, sc[3][y] = a.y >> 16;
+                if (MIN) {
+                    const uint2 b = *(const uint2 *)((const uint16_t *)p.minimum + srow[y] + g);
+                    mn[0][y] = b.x, mn[1][y] = b.x >> 16, mn[2][y] = b.y, mn[3][y] = b.y >> 16;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < SP; j++) {
+                    const int64_t at = srow[y] + min(g + j, groups - 1);
+                    if (p.scale32) {
+                        sc[j][y] = ((const uint32_t *)p.scale)[at];
+                        if (MIN) mn[j][y] = ((const uint32_t *)p.minimum)[at];
+                    } else {
+                        sc[j][y] = ((const uint16_t *)p.scale)[at];
+                        if (MIN) mn[j][y] = ((const uint16_t *)p.minimum)[at];
+                    }
                 }
             }
         }
     };
+    auto value = [&](uint32_t v) { return p.scale32 ? __uint_as_float(v) : fw_to_f32(fw_f16{(uint16_t)v}); };
 
-    for (int s0 = 0; s0 < steps; s0 += csteps) {
-        const int to = min(steps, s0 + csteps);
-        load(s0 + wk, to);
-        if (s0) __syncthreads();
-        // stage x: a unit of 8 inputs per lane, 16 lanes a row's step
-        for (int it = threadIdx.x >> 4; it < rows * (to - s0); it += NTH / 16) {
-            const int r = it % rows, st = it / rows, u = lane & 15; // unit u: block u / 4, part u % 4
-            const int k = (s0 + st) * 128 + (u >> 2) * 32 + (u & 3) * 4;
-            const T *at = (const T *)p.x + (int64_t)(m0 + r) * p.ldx + k;
+    for (int t0 = 0; t0 < turns; t0 += cturns) {
+        const int to = min(turns, t0 + cturns);
+        if (t0 + wk < to) load(t0 + wk);
+        if (t0) __syncthreads();
+        // stage x: a wave per row and turn, a unit of 8 inputs per lane (16 MS units)
+        constexpr int UN = 16 * MS, PER = 64 / UN; // units of a row's turn; rows' turns a wave takes at once
+        for (int it = wave * PER + lane / UN; it < rows * (to - t0); it += NW * PER) {
+            const int r = it % rows, t = it / rows, u = lane % UN;
+            const int blk = (t0 + t) * 4 * MS + (u >> 2);
+            const T *at = (const T *)p.x + (int64_t)(m0 + r) * p.ldx + (blk * 32 + (u & 3) * 4);
+            const bool in = blk < blocks;
             float e[4], h[4];
-            const bool in = (k & ~31) < p.k;
             q4_load4<T>(at, p.vec, in ? 4 : 0, e);
             q4_load4<T>(at + 16, p.vec, in ? 4 : 0, h);
+            if constexpr (CORR) {
+                // sums of the inputs of each group (or part of one, where it is longer than a quarter)
+                float v = ((e[0] + e[1]) + (e[2] + e[3])) + ((h[0] + h[1]) + (h[2] + h[3]));
+                v = v + fw_dpp_f32<FW_DPP_XOR1>(v);
+                v = v + fw_dpp_f32<FW_DPP_XOR2>(v);
+                if (!(fabsf(v) < INFINITY)) odd[r] = 1;
+                if constexpr (GB >= 2 && MS >= 2) v = v + fw_dpp_f32<FW_DPP_HALF_MIRROR>(v);
+                if constexpr (GB >= 4 && MS >= 4) v = v + fw_dpp_f32<FW_DPP_MIRROR>(v);
+                // block b of the turn: quarter b / MS, its scale (b % MS) / GB
+                const int b = u >> 2, j = b % MS / GB;
+                if ((u & 3) == 0 && b % MS % GB == 0) sums[((t * MS + j) * 4 + b / MS) * R + r] = v;
+            }
             if constexpr (F32) {
                 float mx = 0.0f;
 #pragma unroll
@@ -210,6 +249,8 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
                 mx = fmaxf(mx, fw_dpp_f32<FW_DPP_XOR2>(mx));
                 mx = fmaxf(mx, fw_dpp_f32<FW_DPP_HALF_MIRROR>(mx));
                 mx = fmaxf(mx, fw_dpp_f32<FW_DPP_MIRROR>(mx));
+#pragma unroll
+                for (int o = 16; o < UN; o *= 2) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
                 // mx = 1.f x 2^(ex - 127); x is scaled by 2^(14 - (ex - 127)), in two factors that are normal numbers
                 const int ex = max((int)(__float_as_uint(mx) >> 23), 1), up = 141 - ex;
                 const float f1 = __uint_as_float((uint32_t)(127 + up / 2) << 23), f2 = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);
@@ -219,10 +260,10 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
                     h[i] = h[i] * f1 * f2;
                 }
                 // up is -113..140: the inverse 2^-up as a number, subnormal ones included
-                if (u == 0) scal[st * MT * 16 + r] = __builtin_ldexpf(1.0f, -up);
+                if (u == 0) scal[t * R + r] = __builtin_ldexpf(1.0f, -up);
             }
             u4 v = {q4_pair<T>(e[0], e[2]), q4_pair<T>(h[0], h[2]), q4_pair<T>(e[1], e[3]), q4_pair<T>(h[1], h[3])};
-            char *to_lds = xt + r * xrow + st * 256 + u * 16;
+            char *to_lds = xt + r * xrow + t * (256 * MS) + u * 16;
             *(u4 *)to_lds = v;
             if constexpr (F32) {
                 float el[4], hl[4];
@@ -234,96 +275,94 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
                 v = u4{q4_pair<T>(el[0], el[2]), q4_pair<T>(hl[0], hl[2]), q4_pair<T>(el[1], el[3]), q4_pair<T>(hl[1], hl[3])};
                 *(u4 *)(to_lds + plane) = v;
             }
-            if constexpr (CORR) {
-                float t = ((e[0] + e[1]) + (e[2] + e[3])) + ((h[0] + h[1]) + (h[2] + h[3]));
-                t = t + fw_dpp_f32<FW_DPP_XOR1>(t);
-                t = t + fw_dpp_f32<FW_DPP_XOR2>(t);
-                if ((u & 3) == 0) sums[(st * 4 + (u >> 2)) * MT * 16 + r] = t;
-                if (!(fabsf(t) < INFINITY)) odd[r] = 1;
-            }
         }
         __syncthreads();
 
-        for (int s = s0 + wk; s < to; s += U * WK) {
-            u4 w[U][NT];
-            float d[U][NT], e[U][NT];
+        const char *xl[MT]; // this lane's units of each row tile (the last row again behind the end)
 #pragma unroll
-            for (int u = 0; u < U; u++)
+        for (int x = 0; x < MT; x++) xl[x] = xt + min(x * 16 + lr, rows - 1) * xrow + c * 16;
+        for (int t = t0 + wk; t < to; t += WK) {
+            const int tl = t - t0;
+            u4 w[MS][NT];
+            float d[SP][NT];
 #pragma unroll
-                for (int y = 0; y < NT; y++) {
-                    w[u][y] = wq[u][y];
-                    d[u][y] = sc[u][y];
-                    e[u][y] = MIN ? (BF ? fmaf(-128.0f, sc[u][y], mn[u][y]) : mn[u][y]) : -136.0f * sc[u][y];
+            for (int y = 0; y < NT; y++) {
+#pragma unroll
+                for (int u = 0; u < MS; u++) w[u][y] = wq[u][y];
+#pragma unroll
+                for (int j = 0; j < SP; j++) {
+                    // blocks behind the last weigh nothing
+                    const bool in = (t * 4 + c) * MS + j * GB < blocks;
+                    d[j][y] = in ? value(sc[j][y]) : 0.0f;
+                    if constexpr (CORR) {
+                        // what every code is off by, times the inputs' sums: a product over the quarters' groups
+                        float e = MIN ? (in ? value(mn[j][y]) : 0.0f) + (BF ? -128.0f * d[j][y] : 0.0f) : -136.0f * d[j][y];
+                        // (a group longer than a quarter: each quarter has the sum of its own part)
+#pragma unroll
+                        for (int x = 0; x < MT; x++)
+                            acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(sums[((tl * MS + j) * 4 + c) * R + x * 16 + lr], e, acc[x][y], 0, 0, 0);
+                    }
                 }
-            if (s + U * WK < to) load(s + U * WK, to);
+            }
+            if (t + WK < to) load(t + WK);
+            f4 dq[SP][NT];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int st = s + u * WK - s0;
-                if (st >= to - s0) break;
-                f4 dq[NT];
+            for (int y = 0; y < NT; y++)
 #pragma unroll
-                for (int y = 0; y < NT; y++) {
-                    q4_exchange(w[u][y]);
-                    if constexpr (GB == 1) dq[y] = q4_quarters(d[u][y]);
-                }
-                const char *xs = xt + st * 256 + c * 16;
+                for (int j = 0; j < SP; j++) dq[j][y] = q4_quarters(d[j][y]);
+            f4 mid[MT][NT];
+            if constexpr (F32)
 #pragma unroll
                 for (int x = 0; x < MT; x++)
 #pragma unroll
                     for (int y = 0; y < NT; y++) mid[x][y] = f4{};
-                if constexpr (CORR) {
-                    // the inputs' block sums times what every code is off by, four blocks in one product
+            f4 dot[MT][NT];
 #pragma unroll
-                    for (int x = 0; x < MT; x++) {
-                        const float t = sums[(st * 4 + c) * MT * 16 + x * 16 + lr];
+            for (int u = 0; u < MS; u++) {
 #pragma unroll
-                        for (int y = 0; y < NT; y++)
-                            (F32 ? mid[x][y] : acc[x][y]) =
-                                __builtin_amdgcn_mfma_f32_16x16x4f32(t, e[u][y], F32 ? mid[x][y] : acc[x][y], 0, 0, 0);
-                    }
-                }
-                f4 dot[MT][NT];
+                for (int y = 0; y < NT; y++) q4_exchange(w[u][y]);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    u4 b[NT];
+                    const int b = u * 4 + i; // the turn's block
+                    u4 code[NT];
 #pragma unroll
-                    for (int y = 0; y < NT; y++) b[y] = BF ? q4_codes_bf16(w[u][y][i]) : q4_codes_f16<MIN>(w[u][y][i]);
+                    for (int y = 0; y < NT; y++)
+                        code[y] = BF ? q4_codes_bf16(w[u][y][i], magic) : q4_codes_f16<MIN>(w[u][y][i], magic);
 #pragma unroll
                     for (int x = 0; x < MT; x++) {
-                        const int r = min(x * 16 + lr, rows - 1);
-                        const u4 a = *(const u4 *)(xs + r * xrow + i * 64);
+                        const char *at = xl[x] + tl * (256 * MS) + b * 64;
+                        const u4 a = *(const u4 *)at;
                         u4 al;
-                        if constexpr (F32) al = *(const u4 *)(xs + plane + r * xrow + i * 64);
+                        if constexpr (F32) al = *(const u4 *)(at + plane);
 #pragma unroll
                         for (int y = 0; y < NT; y++) {
-                            f4 z = GB == 4 && i ? dot[x][y] : f4{};
+                            f4 z = b % GB ? dot[x][y] : f4{};
                             if constexpr (BF)
-                                z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b[y]), z, 0, 0, 0);
+                                z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, code[y]), z, 0, 0, 0);
                             else {
                                 if constexpr (F32)
-                                    z = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, al), __builtin_bit_cast(h8, b[y]), z, 0, 0, 0);
-                                z = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b[y]), z, 0, 0, 0);
+                                    z = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, al), __builtin_bit_cast(h8, code[y]), z, 0, 0, 0);
+                                z = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, code[y]), z, 0, 0, 0);
                             }
                             dot[x][y] = z;
-                            if (GB == 1 || i == 3) {
-                                const float f = GB == 1 ? dq[y][i] : d[u][y];
-                                f4 &to_acc = F32 ? mid[x][y] : acc[x][y];
+                            if (b % GB == GB - 1 || b == 4 * MS - 1) {
+                                const float f = dq[b % MS / GB][y][b / MS];
+                                f4 &sum = F32 ? mid[x][y] : acc[x][y];
 #pragma unroll
-                                for (int j = 0; j < 4; j++) to_acc[j] = fmaf(f, z[j], to_acc[j]);
+                                for (int j = 0; j < 4; j++) sum[j] = fmaf(f, z[j], sum[j]);
                             }
                         }
                     }
                 }
-                if constexpr (F32) {
+            }
+            if constexpr (F32) {
 #pragma unroll
-                    for (int x = 0; x < MT; x++) {
-                        const f4 f = *(const f4 *)(scal + st * MT * 16 + x * 16 + 4 * c);
+                for (int x = 0; x < MT; x++) {
+                    const f4 f = *(const f4 *)(scal + tl * R + x * 16 + 4 * c);
 #pragma unroll
-                        for (int y = 0; y < NT; y++)
+                    for (int y = 0; y < NT; y++)
 #pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                acc[x][y][j] = fmaf(f[j], mid[x][y][j], acc[x][y][j]);
-                    }
+                        for (int j = 0; j < 4; j++) acc[x][y][j] = fmaf(f[j], mid[x][y][j], acc[x][y][j]);
                 }
             }
         }
@@ -366,34 +405,38 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
     }
 }
 
-template <typename T, bool MIN, int GB, int MT, int NT, int WN, int WK, int U>
+template <typename T, bool MIN, int GB, int MT, int NT, int WN, int WK, int MS>
 static void q4_go(hipStream_t st, Q4P p) {
     constexpr bool CORR = MIN || std::is_same<T, fw_bf16>::value, F32 = std::is_same<T, float>::value;
     const int rows = std::min(p.m, MT * 16);
-    // as many inputs a stage as fit 64 KiB of LDS, a whole number of turns of the waves
-    const int step = Q4X<T>::PARTS * rows * 256 + (CORR ? 256 * MT : 0) + (F32 ? 64 * MT : 0);
+    // as many inputs a stage as fit 64 KiB of LDS, a whole number of turns of every wave
+    const int turn = MS * (Q4X<T>::PARTS * rows * 256 + (CORR ? 256 * MT : 0)) + (F32 ? 64 * MT : 0);
     const int fixed = Q4X<T>::PARTS * rows * 16 + 64 * MT, join = 64 * MT + (WK > 1 ? WN * WK * MT * NT * 1024 : 0);
-    int steps = std::max(1, (65536 - fixed) / step);
-    steps = std::min(steps, (p.k + 127) / 128);
-    if (steps > WK) steps = steps / WK * WK;
-    p.chunk = steps * 128;
-    p.lds = std::max(steps * step + fixed, join);
+    int turns = std::max(1, (65536 - fixed) / turn);
+    turns = std::min(turns, (p.k + 128 * MS - 1) / (128 * MS));
+    if (turns > WK) turns = turns / WK * WK;
+    p.chunk = turns * MS * 128;
+    p.lds = std::max(turns * turn + fixed, join);
     const Q4P all = p;
     for (int64_t at = 0; at < all.m; at += 65535 * 16 * MT) { // the grid's reach in rows
         p.m = (int)std::min<int64_t>(all.m - at, 65535 * 16 * MT);
         p.x = (const T *)all.x + at * all.ldx;
         p.y = (T *)all.y + at * all.ldy;
         const dim3 grid((unsigned)((p.n + 16 * NT * WN - 1) / (16 * NT * WN)), (unsigned)((p.m + 16 * MT - 1) / (16 * MT)));
-        hipLaunchKernelGGL((k_q4<T, MIN, GB, MT, NT, WN, WK, U>), grid, dim3(64 * WN * WK), p.lds, st, p);
+        hipLaunchKernelGGL((k_q4<T, MIN, GB, MT, NT, WN, WK, MS>), grid, dim3(64 * WN * WK), p.lds, st, p);
     }
 }
 template <typename T, bool MIN, int GB>
 static void q4_rows(hipStream_t st, const Q4P &p) {
     const bool wide = p.n >= 16384;
     if (p.m <= 16) {
-        if (wide) q4_go<T, MIN, GB, 1, 1, 4, 2, 2>(st, p);
-        else q4_go<T, MIN, GB, 1, 1, 1, 8, 2>(st, p);
-    } else if (p.m <= 32) q4_go<T, MIN, GB, 2, 1, 4, 1, 2>(st, p);
+#ifndef QA
+#define QA 1, 1, 4, 2, 4
+#define QB 1, 1, 1, 8, 1
+#endif
+        if (wide) q4_go<T, MIN, GB, QA>(st, p);
+        else q4_go<T, MIN, GB, QB>(st, p);
+    } else if (p.m <= 32) q4_go<T, MIN, GB, 2, 1, 4, 1, 4>(st, p);
     else q4_go<T, MIN, GB, 4, 2, 4, 1, 1>(st, p);
 }
 template <typename T>
@@ -401,6 +444,9 @@ static void q4_type(hipStream_t st, const Q4P &p) {
     if (p.group == 128) {
         if (p.minimum) q4_rows<T, true, 4>(st, p);
         else q4_rows<T, false, 4>(st, p);
+    } else if (p.group == 64) {
+        if (p.minimum) q4_rows<T, true, 2>(st, p);
+        else q4_rows<T, false, 2>(st, p);
     } else {
         if (p.minimum) q4_rows<T, true, 1>(st, p);
         else q4_rows<T, false, 1>(st, p);
@@ -433,8 +479,9 @@ extern "C" fwhip_status fwhip_q4_linear(fwhip_ctx *c, const fwhip_q4_linear_args
     if (!dev.ok) return fw_fail(FWHIP_ERR_GENERIC, "fwhip_q4_linear: hipSetDevice failed");
     const int eb = fw_dtype_bytes(a->dtype), vb = 4 * eb;
     const int vec = fw_aligned(a->x, vb) && (a->m == 1 || a->ldx * eb % vb == 0);
+    const int pair = fw_aligned(a->scale, 8) && fw_aligned(a->minimum, 8) && a->k / a->group % 4 == 0;
     const Q4P p = {a->m, a->n, a->k, a->group, a->ldx, a->ldy, a->x, a->q, a->scale, a->minimum, a->bias, a->y,
-                   a->scale_dtype == FWHIP_T_F32, vec, a->group == 32 ? 0 : a->group == 64 ? 1 : 2, 0, 0};
+                   a->scale_dtype == FWHIP_T_F32, vec, pair, 0, 0};
     if (a->dtype == FWHIP_T_F32) q4_type<float>(c->stream, p);
     else if (a->dtype == FWHIP_T_F16) q4_type<fw_f16>(c->stream, p);
     else q4_type<fw_bf16>(c->stream, p);
