@@ -89,30 +89,36 @@ struct Q4X {
     static constexpr int PARTS = std::is_same<T, float>::value ? 2 : 1;
 };
 
+// Four inputs as they lie in memory, and their values.
 template <typename T>
-__device__ __forceinline__ void q4_load4(const T *at, bool vec, int left, float (&v)[4]) {
-    if (vec && left >= 4) {
-        if constexpr (sizeof(T) == 4) {
-            const f4 a = *(const f4 *)at;
+struct Q4Four {
+    typename std::conditional<sizeof(T) == 4, u4, uint2>::type v;
+    __device__ __forceinline__ void load(const T *at, bool vec) {
+        if (vec) v = *(const decltype(v) *)at;
+        else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = a[i];
+            for (int i = 0; i < 4; i++) v[i] = ((const uint32_t *)at)[i];
         } else {
-            const uint2 a = *(const uint2 *)at;
-            v[0] = fw_to_f32(T{(uint16_t)a.x});
-            v[1] = fw_to_f32(T{(uint16_t)(a.x >> 16)});
-            v[2] = fw_to_f32(T{(uint16_t)a.y});
-            v[3] = fw_to_f32(T{(uint16_t)(a.y >> 16)});
+            const uint16_t *a = (const uint16_t *)at;
+            v = make_uint2(a[0] | (uint32_t)a[1] << 16, a[2] | (uint32_t)a[3] << 16);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = i < left ? fw_to_f32(at[i]) : 0.0f;
     }
-}
-template <typename T>
-__device__ __forceinline__ uint32_t q4_pair(float a, float b) {
-    typedef typename std::conditional<std::is_same<T, float>::value, fw_f16, T>::type H;
-    return fw_cvt<H>(a).b | (uint32_t)fw_cvt<H>(b).b << 16;
-}
+    __device__ __forceinline__ void clear() { v = decltype(v){}; }
+    __device__ __forceinline__ float sum(float t) const { // t + the four
+        if constexpr (sizeof(T) == 4) return t + ((__uint_as_float(v[0]) + __uint_as_float(v[1])) + (__uint_as_float(v[2]) + __uint_as_float(v[3])));
+        else if constexpr (std::is_same<T, fw_bf16>::value) {
+            typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+            const b2 one = {(__bf16)1.0f, (__bf16)1.0f};
+            t = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, v.x), one, t, false);
+            return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, v.y), one, t, false);
+        } else {
+            const h2 one = {(_Float16)1.0f, (_Float16)1.0f};
+            t = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, v.x), one, t, false);
+            return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, v.y), one, t, false);
+        }
+    }
+};
+__device__ __forceinline__ uint32_t q4_pair(float a, float b) { return fw_cvt<fw_f16>(a).b | (uint32_t)fw_cvt<fw_f16>(b).b << 16; }
 
 // One output, product by product: w = (code - 8) scale or code scale + minimum.
 template <typename T, bool MIN>
@@ -216,64 +222,80 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
         const int to = min(turns, t0 + cturns);
         if (t0 + wk < to) load(t0 + wk);
         if (t0) __syncthreads();
-        // stage x: a wave per row and turn, a unit of 8 inputs per lane (16 MS units)
-        constexpr int UN = 16 * MS, PER = 64 / UN; // units of a row's turn; rows' turns a wave takes at once
-        for (int it = wave * PER + lane / UN; it < rows * (to - t0); it += NW * PER) {
-            const int r = it % rows, t = it / rows, u = lane % UN;
-            const int blk = (t0 + t) * 4 * MS + (u >> 2);
-            const T *at = (const T *)p.x + (int64_t)(m0 + r) * p.ldx + (blk * 32 + (u & 3) * 4);
-            const bool in = blk < blocks;
-            float e[4], h[4];
-            q4_load4<T>(at, p.vec, in ? 4 : 0, e);
-            q4_load4<T>(at + 16, p.vec, in ? 4 : 0, h);
-            if constexpr (CORR) {
-                // sums of the inputs of each group (or part of one, where it is longer than a quarter)
-                float v = ((e[0] + e[1]) + (e[2] + e[3])) + ((h[0] + h[1]) + (h[2] + h[3]));
-                v = v + fw_dpp_f32<FW_DPP_XOR1>(v);
-                v = v + fw_dpp_f32<FW_DPP_XOR2>(v);
-                if (!(fabsf(v) < INFINITY)) odd[r] = 1;
-                if constexpr (GB >= 2 && MS >= 2) v = v + fw_dpp_f32<FW_DPP_HALF_MIRROR>(v);
-                if constexpr (GB >= 4 && MS >= 4) v = v + fw_dpp_f32<FW_DPP_MIRROR>(v);
-                // block b of the turn: quarter b / MS, its scale (b % MS) / GB
-                const int b = u >> 2, j = b % MS / GB;
-                if ((u & 3) == 0 && b % MS % GB == 0) sums[((t * MS + j) * 4 + b / MS) * R + r] = v;
+        // stage x: a unit of 8 inputs per lane, 16 MS of them a row's turn; four
+        // row's turns are on their way from memory at once
+        constexpr int UN = 16 * MS, PER = NW * 64 / UN, AT = 4;
+        const int items = rows * (to - t0), u = lane % UN;
+        const float per_row = 1.0f / (float)rows; // (i + 1/2) / rows, cut, is i / rows: items stay below 2^16
+        for (int i0 = threadIdx.x / UN; i0 < items; i0 += AT * PER) {
+            Q4Four<T> xe[AT], xh[AT];
+            int row[AT], turn[AT];
+#pragma unroll
+            for (int j = 0; j < AT; j++) {
+                const int it = min(i0 + j * PER, items - 1);
+                turn[j] = (int)(((float)it + 0.5f) * per_row);
+                row[j] = it - turn[j] * rows;
+                const int blk = min((t0 + turn[j]) * 4 * MS + (u >> 2), blocks - 1);
+                const T *at = (const T *)p.x + (int64_t)(m0 + row[j]) * p.ldx + (blk * 32 + (u & 3) * 4);
+                xe[j].load(at, p.vec);
+                xh[j].load(at + 16, p.vec);
             }
-            if constexpr (F32) {
-                float mx = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    mx = fmaxf(mx, fabsf(e[i]) < INFINITY ? fabsf(e[i]) : 0.0f);
-                    mx = fmaxf(mx, fabsf(h[i]) < INFINITY ? fabsf(h[i]) : 0.0f);
+            for (int j = 0; j < AT; j++) {
+                if (i0 + j * PER >= items) break;
+                const int r = row[j], t = turn[j];
+                if ((t0 + t) * 4 * MS + (u >> 2) >= blocks) {
+                    xe[j].clear();
+                    xh[j].clear();
                 }
-                mx = fmaxf(mx, fw_dpp_f32<FW_DPP_XOR1>(mx));
-                mx = fmaxf(mx, fw_dpp_f32<FW_DPP_XOR2>(mx));
-                mx = fmaxf(mx, fw_dpp_f32<FW_DPP_HALF_MIRROR>(mx));
-                mx = fmaxf(mx, fw_dpp_f32<FW_DPP_MIRROR>(mx));
-#pragma unroll
-                for (int o = 16; o < UN; o *= 2) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-                // mx = 1.f x 2^(ex - 127); x is scaled by 2^(14 - (ex - 127)), in two factors that are normal numbers
-                const int ex = max((int)(__float_as_uint(mx) >> 23), 1), up = 141 - ex;
-                const float f1 = __uint_as_float((uint32_t)(127 + up / 2) << 23), f2 = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    e[i] = e[i] * f1 * f2;
-                    h[i] = h[i] * f1 * f2;
+                if constexpr (CORR) {
+                    // sums of the inputs of each group (or part of one, where it is longer than a quarter)
+                    float v = xh[j].sum(xe[j].sum(0.0f));
+                    v = v + fw_dpp_f32<FW_DPP_XOR1>(v);
+                    v = v + fw_dpp_f32<FW_DPP_XOR2>(v);
+                    if (!(fabsf(v) < INFINITY)) odd[r] = 1;
+                    if constexpr (GB >= 2 && MS >= 2) v = v + fw_dpp_f32<FW_DPP_HALF_MIRROR>(v);
+                    if constexpr (GB >= 4 && MS >= 4) v = v + fw_dpp_f32<FW_DPP_MIRROR>(v);
+                    // block b of the turn: quarter b / MS, its scale (b % MS) / GB
+                    const int b = u >> 2;
+                    if ((u & 3) == 0 && b % MS % GB == 0) sums[((t * MS + b % MS / GB) * 4 + b / MS) * R + r] = v;
                 }
-                // up is -113..140: the inverse 2^-up as a number, subnormal ones included
-                if (u == 0) scal[t * R + r] = __builtin_ldexpf(1.0f, -up);
-            }
-            u4 v = {q4_pair<T>(e[0], e[2]), q4_pair<T>(h[0], h[2]), q4_pair<T>(e[1], e[3]), q4_pair<T>(h[1], h[3])};
-            char *to_lds = xt + r * xrow + t * (256 * MS) + u * 16;
-            *(u4 *)to_lds = v;
-            if constexpr (F32) {
-                float el[4], hl[4];
+                char *to_lds = xt + r * xrow + t * (256 * MS) + u * 16;
+                if constexpr (F32) {
+                    float e[4], h[4], el[4], hl[4], mx = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; i++) { // parts of values that are not finite: nothing more
-                    el[i] = fabsf(e[i]) < INFINITY ? e[i] - (float)(_Float16)e[i] : 0.0f;
-                    hl[i] = fabsf(h[i]) < INFINITY ? h[i] - (float)(_Float16)h[i] : 0.0f;
+                    for (int i = 0; i < 4; i++) {
+                        e[i] = __uint_as_float(xe[j].v[i]);
+                        h[i] = __uint_as_float(xh[j].v[i]);
+                        mx = fmaxf(mx, fabsf(e[i]) < INFINITY ? fabsf(e[i]) : 0.0f);
+                        mx = fmaxf(mx, fabsf(h[i]) < INFINITY ? fabsf(h[i]) : 0.0f);
+                    }
+                    mx = fmaxf(mx, fw_dpp_f32<FW_DPP_XOR1>(mx));
+                    mx = fmaxf(mx, fw_dpp_f32<FW_DPP_XOR2>(mx));
+                    mx = fmaxf(mx, fw_dpp_f32<FW_DPP_HALF_MIRROR>(mx));
+                    mx = fmaxf(mx, fw_dpp_f32<FW_DPP_MIRROR>(mx));
+#pragma unroll
+                    for (int o = 16; o < UN; o *= 2) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+                    // mx = 1.f x 2^(ex - 127); x is scaled by 2^(14 - (ex - 127)), in two factors that are normal numbers
+                    const int ex = max((int)(__float_as_uint(mx) >> 23), 1), up = 141 - ex;
+                    const float f1 = __uint_as_float((uint32_t)(127 + up / 2) << 23), f2 = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        e[i] = e[i] * f1 * f2;
+                        h[i] = h[i] * f1 * f2;
+                        // second parts; of values that are not finite: nothing more
+                        el[i] = fabsf(e[i]) < INFINITY ? e[i] - (float)(_Float16)e[i] : 0.0f;
+                        hl[i] = fabsf(h[i]) < INFINITY ? h[i] - (float)(_Float16)h[i] : 0.0f;
+                    }
+                    // up is -113..140: the inverse 2^-up as a number, subnormal ones included
+                    if (u == 0) scal[t * R + r] = __builtin_ldexpf(1.0f, -up);
+                    *(u4 *)to_lds = u4{q4_pair(e[0], e[2]), q4_pair(h[0], h[2]), q4_pair(e[1], e[3]), q4_pair(h[1], h[3])};
+                    *(u4 *)(to_lds + plane) = u4{q4_pair(el[0], el[2]), q4_pair(hl[0], hl[2]), q4_pair(el[1], el[3]), q4_pair(hl[1], hl[3])};
+                } else {
+                    const uint2 e = xe[j].v, h = xh[j].v;
+                    *(u4 *)to_lds = u4{__builtin_amdgcn_perm(e.y, e.x, 0x05040100), __builtin_amdgcn_perm(h.y, h.x, 0x05040100),
+                                       __builtin_amdgcn_perm(e.y, e.x, 0x07060302), __builtin_amdgcn_perm(h.y, h.x, 0x07060302)};
                 }
-                v = u4{q4_pair<T>(el[0], el[2]), q4_pair<T>(hl[0], hl[2]), q4_pair<T>(el[1], el[3]), q4_pair<T>(hl[1], hl[3])};
-                *(u4 *)(to_lds + plane) = v;
             }
         }
         __syncthreads();
@@ -426,18 +448,33 @@ static void q4_go(hipStream_t st, Q4P p) {
         hipLaunchKernelGGL((k_q4<T, MIN, GB, MT, NT, WN, WK, MS>), grid, dim3(64 * WN * WK), p.lds, st, p);
     }
 }
+// Which form runs.  x is staged once a block, so many outputs a block save
+// staging; few outputs a block spread a small weight over the chip, its waves
+// then sharing outputs and taking turns of the inputs.  Longer turns (512
+// inputs, not 128) carry fewer scale loads and waits but leave more idle at the
+// end of short rows.  Measured both sides of each border, us, this form / the next:
+//   1..16 rows, up to 640 tiles of 16 outputs: 1 x 5120 x 1280 5.2 / 7.9
+//     k < 2048: 10 x 51866 x 1280 (f32) 18.5 / 32;  1 x 51866 x 1280 13.1 / 20
+//     up to 1280 tiles: 8 x 14336 x 4096 14.3 / 18.8;  above: 16 x 28672 x 8192 49 / 44
+//   17..32 rows: 20 x 1280 x 1280 7.3 / 8.0;  32 x 5120 x 1280 (f32) 15.9 / 21;  32 x 28672 x 8192 99 / 63
+//   more, in tiles of 64 rows, by how many blocks there are: 1500 x 5120 x 1280 58 / 70;
+//     256 x 5120 x 5120 106 / 90;  64 x 5120 x 5120 70 / 50
 template <typename T, bool MIN, int GB>
 static void q4_rows(hipStream_t st, const Q4P &p) {
-    const bool wide = p.n >= 16384;
+    const int64_t tiles = (p.n + 15) / 16, mt = (p.m + 63) / 64;
     if (p.m <= 16) {
-#ifndef QA
-#define QA 1, 1, 4, 2, 4
-#define QB 1, 1, 1, 8, 1
-#endif
-        if (wide) q4_go<T, MIN, GB, QA>(st, p);
-        else q4_go<T, MIN, GB, QB>(st, p);
-    } else if (p.m <= 32) q4_go<T, MIN, GB, 2, 1, 4, 1, 4>(st, p);
-    else q4_go<T, MIN, GB, 4, 2, 4, 1, 1>(st, p);
+        if (tiles <= 640) q4_go<T, MIN, GB, 1, 1, 1, 8, 1>(st, p);
+        else if (p.k < 2048) q4_go<T, MIN, GB, 1, 1, 8, 1, 2>(st, p);
+        else if (tiles <= 1280) q4_go<T, MIN, GB, 1, 1, 4, 2, 4>(st, p);
+        else q4_go<T, MIN, GB, 1, 1, 8, 1, 4>(st, p);
+    } else if (p.m <= 32) {
+        if (tiles <= 128) q4_go<T, MIN, GB, 2, 1, 1, 8, 1>(st, p);
+        else if (tiles <= 512) q4_go<T, MIN, GB, 2, 1, 2, 4, 1>(st, p);
+        else q4_go<T, MIN, GB, 2, 1, 8, 1, 2>(st, p);
+    } else if ((tiles + 15) / 16 * mt >= 256) q4_go<T, MIN, GB, 4, 2, 8, 1, 1>(st, p);
+    else if ((tiles + 7) / 8 * mt >= 128) q4_go<T, MIN, GB, 4, 1, 8, 1, 2>(st, p);
+    else if ((tiles + 3) / 4 * mt >= 96) q4_go<T, MIN, GB, 4, 1, 4, 2, 2>(st, p);
+    else q4_go<T, MIN, GB, 4, 1, 2, 4, 1>(st, p);
 }
 template <typename T>
 static void q4_type(hipStream_t st, const Q4P &p) {
