@@ -198,47 +198,78 @@ extern "C" fwhip_status fwhip_paged_plan(fwhip_ctx *c, const fwhip_paged_plan_ar
     p.slot = a->slot;
     p.mask = a->mask;
     p.status = a->status;
+    // Few requests with many rows or long tables (prompts): several blocks a
+    // request, each with a slice.  Many requests: several a block, which bounds
+    // how often the lengths before a block are summed.
     p.rpb = 1 + a->n_req / 2048;
     const int blocks = a->n_req ? (a->n_req + p.rpb - 1) / p.rpb : 1;
-    hipLaunchKernelGGL(k_paged_plan, dim3(blocks, 1), dim3(PLAN_T), 0, c->stream, p);
+    const int64_t work = ((int64_t)a->n_rows / std::max(a->n_req, 1) + a->width) / PLAN_T;
+    const int slices = (int)std::max<int64_t>(1, std::min<int64_t>(work / 4, std::max(1, 1024 / blocks)));
+    hipLaunchKernelGGL(k_paged_plan, dim3(blocks, slices), dim3(PLAN_T), 0, c->stream, p);
     return fw_launched("fwhip_paged_plan");
 }
 
 // ---------------------------------------------------------------------------
 // append
+// A block per row: its K and V in pieces of VEC elements, 16 bytes or more of each
+// where the addresses allow (VEC = 8), element by element where not.  Bound by
+// the rows' bytes, read once and written once.
 struct AppendP {
-    int64_t n; // elements of K (and of V)
-    int heads, dim;
+    int rows, pieces, per_head; // pieces of K in a row, and in a head
+    FwDiv head;                 // by per_head
     int64_t k_row, k_head, v_row, v_head, page_stride, token_stride, head_stride, slots;
-    FwDiv page;
+    int page;
     const void *k, *v;
     const int64_t *slot;
     void *kc, *vc;
 };
 
-template <typename S, typename D>
+template <typename S, typename D, int VEC>
+__device__ __forceinline__ void append_piece(const S *from, D *to) {
+    struct alignas(VEC == 1 ? sizeof(S) : 16) In {
+        S v[VEC];
+    };
+    struct alignas(VEC == 1 ? sizeof(D) : 16) Out {
+        D v[VEC];
+    };
+    const In a = *(const In *)from;
+    Out b;
+#pragma unroll
+    for (int i = 0; i < VEC; i++) b.v[i] = fw_cvt<D>(fw_to_f32(a.v[i]));
+    *(Out *)to = b;
+}
+template <typename S, typename D, int VEC>
 __global__ void __launch_bounds__(256) k_paged_append(AppendP p) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.n; i += (int64_t)gridDim.x * 256) {
-        const int e = (int)(i % p.dim), h = (int)(i / p.dim % p.heads);
-        const int64_t row = i / p.dim / p.heads, slot = p.slot[row];
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const int64_t slot = p.slot[row];
         if (slot < 0 || slot >= p.slots) continue;
-        const int64_t pg = slot / p.page.d, off = slot % p.page.d;
-        const int64_t to = pg * p.page_stride + off * p.token_stride + h * p.head_stride + e;
-        ((D *)p.kc)[to] = fw_cvt<D>(fw_to_f32(((const S *)p.k)[row * p.k_row + h * p.k_head + e]));
-        ((D *)p.vc)[to] = fw_cvt<D>(fw_to_f32(((const S *)p.v)[row * p.v_row + h * p.v_head + e]));
+        const int64_t to = slot / p.page * p.page_stride + slot % p.page * p.token_stride;
+        for (int64_t i = threadIdx.x; i < 2 * (int64_t)p.pieces; i += blockDim.x) {
+            const bool v = i >= p.pieces;
+            const uint32_t at = (uint32_t)(v ? i - p.pieces : i), h = fw_div(at, p.head);
+            const int64_t e = (int64_t)(at - h * p.per_head) * VEC;
+            if (v) append_piece<S, D, VEC>((const S *)p.v + row * p.v_row + h * p.v_head + e, (D *)p.vc + to + h * p.head_stride + e);
+            else append_piece<S, D, VEC>((const S *)p.k + row * p.k_row + h * p.k_head + e, (D *)p.kc + to + h * p.head_stride + e);
+        }
     }
 }
 
-template <typename S, typename D>
+template <typename S, typename D, int VEC>
 static void append_launch(hipStream_t st, const AppendP &p) {
-    const int64_t blocks = std::min<int64_t>((p.n + 255) / 256, 1 << 20);
-    hipLaunchKernelGGL((k_paged_append<S, D>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+    const int threads = (int)std::min<int64_t>(256, (2 * (int64_t)p.pieces + 63) / 64 * 64);
+    hipLaunchKernelGGL((k_paged_append<S, D, VEC>), dim3((unsigned)std::min(p.rows, 1 << 20)), dim3(threads), 0, st, p);
 }
-template <typename S>
+template <typename S, int VEC>
 static void append_to(hipStream_t st, int dtype, const AppendP &p) {
-    if (dtype == FWHIP_T_F32) append_launch<S, float>(st, p);
-    else if (dtype == FWHIP_T_F16) append_launch<S, fw_f16>(st, p);
-    else append_launch<S, fw_bf16>(st, p);
+    if (dtype == FWHIP_T_F32) append_launch<S, float, VEC>(st, p);
+    else if (dtype == FWHIP_T_F16) append_launch<S, fw_f16, VEC>(st, p);
+    else append_launch<S, fw_bf16, VEC>(st, p);
+}
+template <int VEC>
+static void append_from(hipStream_t st, int src, int dst, const AppendP &p) {
+    if (src == FWHIP_T_F32) append_to<float, VEC>(st, dst, p);
+    else if (src == FWHIP_T_F16) append_to<fw_f16, VEC>(st, dst, p);
+    else append_to<fw_bf16, VEC>(st, dst, p);
 }
 
 extern "C" fwhip_status fwhip_paged_append(fwhip_ctx *c, const fwhip_paged_append_args *a) {
@@ -264,10 +295,18 @@ extern "C" fwhip_status fwhip_paged_append(fwhip_ctx *c, const fwhip_paged_appen
     if (a->n_rows == 0 || a->n_pages == 0) return FWHIP_OK;
     FwOnDevice dev(c);
     if (!dev.ok) return fw_fail(FWHIP_ERR_GENERIC, "fwhip_paged_append: hipSetDevice failed");
+    // pieces of 8 elements where every address of one is a multiple of 16 bytes
+    const int sb = fw_dtype_bytes(a->src_dtype), db = fw_dtype_bytes(a->cache_dtype);
+    bool wide = a->head_dim % 8 == 0 && fw_aligned(a->k, 16) && fw_aligned(a->v, 16) && fw_aligned(a->k_cache, 16) &&
+                fw_aligned(a->v_cache, 16);
+    for (int64_t s : {a->k_row, a->k_head, a->v_row, a->v_head}) wide = wide && s * sb % 16 == 0;
+    for (int64_t s : {a->page_stride, a->token_stride, a->head_stride}) wide = wide && s * db % 16 == 0;
+    const int vec = wide ? 8 : 1;
     AppendP p;
-    p.n = (int64_t)a->n_rows * a->n_heads * a->head_dim;
-    p.heads = a->n_heads;
-    p.dim = a->head_dim;
+    p.rows = a->n_rows;
+    p.per_head = a->head_dim / vec;
+    p.pieces = a->n_heads * p.per_head;
+    p.head = fw_div_make((uint32_t)p.per_head);
     p.k_row = a->k_row;
     p.k_head = a->k_head;
     p.v_row = a->v_row;
@@ -276,14 +315,13 @@ extern "C" fwhip_status fwhip_paged_append(fwhip_ctx *c, const fwhip_paged_appen
     p.token_stride = a->token_stride;
     p.head_stride = a->head_stride;
     p.slots = (int64_t)a->n_pages * a->page_size;
-    p.page = fw_div_make((uint32_t)a->page_size);
+    p.page = a->page_size;
     p.k = a->k;
     p.v = a->v;
     p.slot = a->slot;
     p.kc = a->k_cache;
     p.vc = a->v_cache;
-    if (a->src_dtype == FWHIP_T_F32) append_to<float>(c->stream, a->cache_dtype, p);
-    else if (a->src_dtype == FWHIP_T_F16) append_to<fw_f16>(c->stream, a->cache_dtype, p);
-    else append_to<fw_bf16>(c->stream, a->cache_dtype, p);
+    if (wide) append_from<8>(c->stream, a->src_dtype, a->cache_dtype, p);
+    else append_from<1>(c->stream, a->src_dtype, a->cache_dtype, p);
     return fw_launched("fwhip_paged_append");
 }

@@ -102,7 +102,7 @@ def plan_inputs(rng, n_req, ctx, new, page, extra_width, spare, tree):
 @pytest.mark.parametrize("n_req,ctx,new,page,tree,words", [
     (1, 0, 1, 16, False, 0), (1, 30, 8, 16, True, 1), (3, 50, 5, 1, True, 1), (10, 440, 8, 16, True, 1),
     (64, 3000, 64, 24, True, 1), (33, 700, 130, 64, True, 3), (7, 100, 256, 16, True, 4), (5, 90, 1000, 16, False, 0),
-    (300, 900, 17, 32, True, 2), (5000, 64, 3, 16, True, 1), (1, 10, 20000, 16, False, 0)])
+    (300, 900, 17, 32, True, 2), (5000, 64, 3, 16, True, 1), (1, 10, 20000, 16, False, 0), (2, 9000, 64, 1, True, 1), (3, 40, 3000, 16, False, 0)])
 def test_plan(tctx, n_req, ctx, new, page, tree, words):
     rng = np.random.default_rng(n_req * 7 + new)
     lens, n_new, table, held, free, parents = plan_inputs(rng, n_req, ctx, new, page, 3, 100000, tree)
