@@ -16,6 +16,7 @@
 // of each request's rows and table columns.
 struct PlanP {
     int n_req, width, n_rows, n_free, words, rpb;
+    int quads; // table rows in 16-byte pieces
     FwDiv page;
     const int32_t *len, *n_new, *parents, *table, *held, *free_pages, *free_count;
     int32_t *table_out, *held_out, *count_out, *row_start, *row_req, *pos;
@@ -108,12 +109,24 @@ __global__ void __launch_bounds__(PLAN_T) k_paged_plan(PlanP p) {
 
         const int32_t *trow = p.table + (int64_t)r * p.width;
         int32_t *orow = p.table_out + (int64_t)r * p.width;
-        const bool copy = p.table != p.table_out;
-        for (int64_t c = blockIdx.y * PLAN_T + t; c < p.width; c += gridDim.y * PLAN_T) {
-            const bool is_new = c >= held && c < held + take;
-            if (is_new) orow[c] = fresh[-(c - held)];
-            else if (copy) orow[c] = trow[c];
-        }
+        if (p.table != p.table_out) {
+            if (p.quads)
+                for (int64_t c = blockIdx.y * PLAN_T + t; c < p.width / 4; c += gridDim.y * PLAN_T) {
+                    int4 v = ((const int4 *)trow)[c];
+                    if (take && 4 * c + 3 >= held && 4 * c < held + take) {
+                        int e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (4 * c + i >= held && 4 * c + i < held + take) e[i] = fresh[-(4 * c + i - held)];
+                        v = make_int4(e[0], e[1], e[2], e[3]);
+                    }
+                    ((int4 *)orow)[c] = v;
+                }
+            else
+                for (int64_t c = blockIdx.y * PLAN_T + t; c < p.width; c += gridDim.y * PLAN_T)
+                    orow[c] = c >= held && c < held + take ? fresh[-(c - held)] : trow[c];
+        } else
+            for (int64_t c = blockIdx.y * PLAN_T + t; c < take; c += gridDim.y * PLAN_T) orow[held + c] = fresh[-c];
         const bool tree = p.words > 0;
         const bool fits = !tree || q.rows <= (int64_t)64 * p.words;
         for (int64_t i = blockIdx.y * PLAN_T + t; i < n; i += gridDim.y * PLAN_T) {
@@ -201,6 +214,7 @@ extern "C" fwhip_status fwhip_paged_plan(fwhip_ctx *c, const fwhip_paged_plan_ar
     // Few requests with many rows or long tables (prompts): several blocks a
     // request, each with a slice.  Many requests: several a block, which bounds
     // how often the lengths before a block are summed.
+    p.quads = a->width % 4 == 0 && fw_aligned(a->table, 16) && fw_aligned(a->table_out, 16);
     p.rpb = 1 + a->n_req / 2048;
     const int blocks = a->n_req ? (a->n_req + p.rpb - 1) / p.rpb : 1;
     const int64_t work = ((int64_t)a->n_rows / std::max(a->n_req, 1) + a->width) / PLAN_T;
