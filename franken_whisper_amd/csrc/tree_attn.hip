@@ -112,24 +112,13 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// Weights are 2^15 e^(z - m): the factor cancels in o / l and keeps f16 weights
-// of far smaller keys (down to 2^-29 of the largest) in the normal range.
-#define TREE_BIAS 15.0f
+// Weights are 2^7 2^(z - m) with m the largest score so far, up to a slack of 8:
+// while a new largest stays within it, m stays, what is there need not be
+// scaled, and no weight passes 2^15 (an f16 holds 65504).  The factor cancels in
+// o / l; it keeps f16 weights of far smaller keys (down to 2^-21 of 2^m) normal.
+#define TREE_BIAS 7.0f
+#define TREE_SLACK 8.0f
 __device__ __forceinline__ float tree_base(float m) { return m == -INFINITY ? 0.0f : m - TREE_BIAS; }
-
-template <typename T>
-__device__ __forceinline__ u4 drop_nonfinite(u4 v) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if constexpr (sizeof(T) == 4) v[i] = (v[i] & 0x7f800000u) == 0x7f800000u ? 0 : v[i];
-        else {
-            constexpr uint32_t E = std::is_same<T, fw_f16>::value ? 0x7c00u : 0x7f80u;
-            if ((v[i] & E) == E) v[i] &= 0xffff0000u;
-            if ((v[i] >> 16 & E) == E) v[i] &= 0xffffu;
-        }
-    }
-    return v;
-}
 
 // What a block finds about its request; bad: out of the call's bounds.
 struct TreeReq {
@@ -143,6 +132,13 @@ __device__ __forceinline__ TreeReq tree_req(const TreeP &p, int r) {
     q.len = p.len[r];
     q.bad = q.len < 0 || q.n > p.max_new || (int64_t)q.len + q.n > p.max_len;
     return q;
+}
+// Whether new token i of the request sees key j < last.
+__device__ __forceinline__ bool tree_sees(const TreeP &p, const TreeReq &q, int i, int j, int last) {
+    const int t = j - q.len;
+    bool yes = j < last;
+    if (yes && t >= 0) yes = p.words ? p.mask[(int64_t)(q.row0 + i) * p.words + (t >> 6)] >> (t & 63) & 1 : t <= i;
+    return yes;
 }
 // Whether new token i of a request with n of them sees any key.
 __device__ __forceinline__ bool tree_sees_any(const TreeP &p, const TreeReq &q, int i) {
@@ -230,48 +226,52 @@ struct Rows {
             for (int d = 0; d < DT; d++) o[x][d] = f4{};
         }
     }
-    // Products of the step at key j to -inf where a row does not see the key; the
-    // keys it sees as bits (4 per key tile).
-    __device__ __forceinline__ uint32_t mask(const TreeP &p, const TreeReq &rq, int x, int j, int last, f4 (&z)[KT]) const {
+    // Products of the step at key j to -inf where a row does not see the key.
+    __device__ __forceinline__ void mask(const TreeP &p, const TreeReq &rq, int x, int j, int last, f4 (&z)[KT]) const {
         const int c = (threadIdx.x & 63) >> 4;
-        uint32_t sees = 0;
 #pragma unroll
         for (int k = 0; k < KT; k++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int key = j + k * 16 + 4 * c + i, t = key - rq.len;
-                bool yes = key < last;
-                if (yes && t >= 0)
-                    yes = p.words ? p.mask[(int64_t)(rq.row0 + node[x]) * p.words + (t >> 6)] >> (t & 63) & 1 : t <= node[x];
-                if (!yes) z[k][i] = -INFINITY;
-                sees |= (uint32_t)yes << (4 * k + i);
-            }
-        return sees;
+            for (int i = 0; i < 4; i++)
+                if (!tree_sees(p, rq, node[x], j + k * 16 + 4 * c + i, last)) z[k][i] = -INFINITY;
     }
-    // Products q . k to weights (in place); what is there already is scaled to the new maximum.
-    __device__ __forceinline__ void weigh(int x, f4 (&z)[KT], float zs) {
-        float mx = z[0][0];
+    // Products q . k to weights (in place); what is there already is scaled where the maximum moves.
+    __device__ __forceinline__ void weigh(f4 (&z)[RT][KT], float zs) {
+        float mx[RT];
+        bool moves = false;
 #pragma unroll
-        for (int k = 0; k < KT; k++)
+        for (int x = 0; x < RT; x++) {
+            mx[x] = z[x][0][0];
 #pragma unroll
-            for (int i = 0; i < 4; i++) mx = fmaxf(mx, z[k][i]);
-        mx = quarters_max(mx) * zs;
-        if (__any(mx > m[x])) {
-            const float mn = fmaxf(mx, m[x]), f = __builtin_amdgcn_exp2f(m[x] - TREE_BIAS - tree_base(mn));
-            m[x] = mn;
-            l[x] *= f;
+            for (int k = 0; k < KT; k++)
 #pragma unroll
-            for (int d = 0; d < DT; d++) o[x][d] *= f;
+                for (int i = 0; i < 4; i++) mx[x] = fmaxf(mx[x], z[x][k][i]);
+            mx[x] = quarters_max(mx[x]) * zs;
+            moves |= mx[x] > m[x] + TREE_SLACK;
         }
-        const float base = tree_base(m[x]);
+        if (__any(moves)) {
 #pragma unroll
-        for (int k = 0; k < KT; k++)
+            for (int x = 0; x < RT; x++) {
+                const float mn = mx[x] > m[x] + TREE_SLACK ? mx[x] : m[x];
+                const float f = __builtin_amdgcn_exp2f(m[x] - TREE_BIAS - tree_base(mn));
+                m[x] = mn;
+                l[x] *= f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                // rounded before the difference, as the maximum is: its own weight is exact at any size
-                z[k][i] = __builtin_amdgcn_exp2f(z[k][i] * zs - base);
-                l[x] += z[k][i];
+                for (int d = 0; d < DT; d++) o[x][d] *= f;
             }
+        }
+#pragma unroll
+        for (int x = 0; x < RT; x++) {
+            const float base = tree_base(m[x]);
+#pragma unroll
+            for (int k = 0; k < KT; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    // rounded before the difference, as the maximum is: its own weight is exact at any size
+                    z[x][k][i] = __builtin_amdgcn_exp2f(z[x][k][i] * zs - base);
+                    l[x] += z[x][k][i];
+                }
+        }
     }
     // o += weights times the V tile in LDS (rows of VROW bytes).
     template <int VROW>
@@ -303,33 +303,6 @@ struct Rows {
                     for (int x = 0; x < RT; x++)
                         o[x][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, w[x][0][i], o[x][d], 0, 0, 0);
                 }
-            }
-        }
-    }
-    // The values of V that are not finite, for the rows that see them (they were
-    // left out of the tile).
-    __device__ __forceinline__ void add_dropped(const TreeP &p, const int32_t *trow, int kvh, int j, int last,
-                                             const f4 (&w)[RT][KT], const uint32_t (&sees)[RT]) {
-        const int lane = threadIdx.x & 63, lr = lane & 15, c = lane >> 4;
-        for (int key = 0; key < KEYS && j + key < last; key++) {
-            const int from = ((key & 15) >> 2) * 16 + lr, slot = (key >> 4) * 4 + (key & 3);
-            const int32_t id = trow[fw_div((uint32_t)(j + key), p.page)];
-            if ((uint32_t)id >= (uint32_t)p.n_pages) continue;
-            const T *v = (const T *)((const char *)((const T *)p.vc + kvh * p.head_stride) + tree_at(p, j + key, id));
-#pragma unroll
-            for (int x = 0; x < RT; x++) {
-                float mine = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4 * KT; i++) mine = i == slot ? w[x][i >> 2][i & 3] : mine;
-                mine = __shfl(mine, from);
-                const bool yes = __shfl((int)sees[x], from) >> slot & 1;
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float a = fw_to_f32(v[16 * d + 4 * c + i]);
-                        if (yes && !(fabsf(a) < INFINITY)) o[x][d][i] += mine * a;
-                    }
             }
         }
     }
@@ -448,6 +421,71 @@ struct TreeBlock {
     }
 };
 
+// A block's rows once more, one row a wave at a time and key by key, after
+// outputs that are not finite: those may come from values that a row does not see
+// (0 times infinity) or from the halves of a weight (infinity less infinity),
+// which do not meet here.  lds: 4 x (D + 192) floats.
+template <typename T, int D>
+__device__ __forceinline__ void tree_slow(const TreeP &p, const TreeBlock &b, char *lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float *sq = (float *)lds + wave * (D + 192), *sp = sq + D;
+    int64_t *sat = (int64_t *)(sp + 64);
+    const int32_t *trow = p.table + (int64_t)b.r * p.table_stride;
+    const char *kbase = (const char *)((const T *)p.kc + b.kvh * p.head_stride);
+    const char *vbase = (const char *)((const T *)p.vc + b.kvh * p.head_stride);
+    for (int t = b.t0 + wave; t < min(b.t0 + p.tile_rows, b.total); t += 4) {
+        const int i = t / b.group, h = b.kvh * b.group + t % b.group;
+        const T *q = (const T *)p.q + (int64_t)(b.rq.row0 + i) * p.q_row + h * p.q_head;
+        wave_fence();
+        for (int e = lane; e < D; e += 64) sq[e] = fw_to_f32(q[e]);
+        wave_fence();
+        float m = -INFINITY, l = 0.0f, o[D / 64] = {};
+        for (int j0 = b.first; j0 < b.last; j0 += 64) {
+            const int j = j0 + lane;
+            const bool yes = tree_sees(p, b.rq, i, j, b.last);
+            float z = -INFINITY;
+            int64_t at = -2; // not seen; -1: no page
+            if (yes) {
+                const int32_t id = trow[fw_div((uint32_t)j, p.page)];
+                at = (uint32_t)id < (uint32_t)p.n_pages ? (int64_t)tree_at(p, j, id) : -1;
+                z = at < 0 ? __builtin_nanf("") : 0.0f;
+                if (at >= 0)
+                    for (int e = 0; e < D; e++) z = fmaf(sq[e], fw_to_f32(((const T *)(kbase + at))[e]), z);
+                z = z * (p.scale * 1.44269504088896340736f);
+            }
+            if (!__any(yes)) continue;
+            const float mn = fmaxf(m, fw_wave_max(z)), base = tree_base(mn);
+            const float w = yes ? __builtin_amdgcn_exp2f(z - base) : 0.0f, f = __builtin_amdgcn_exp2f(m - TREE_BIAS - base);
+            l = l * f + fw_wave_sum(w);
+            m = mn;
+            sp[lane] = w;
+            sat[lane] = at;
+            wave_fence();
+            for (int x = 0; x < D / 64; x++) {
+                float a = f == 1.0f ? o[x] : o[x] * f;
+                for (int k = 0; k < 64; k++)
+                    if (sat[k] >= 0) a = fmaf(sp[k], fw_to_f32(((const T *)(vbase + sat[k]))[x * 64 + lane]), a);
+                    else if (sat[k] == -1) a += sp[k]; // NaN
+                o[x] = a;
+            }
+            wave_fence();
+        }
+        if (b.whole) {
+            T *out = (T *)p.out + (int64_t)(b.rq.row0 + i) * p.out_row + h * p.out_head;
+            const bool any = tree_sees_any(p, b.rq, i);
+            for (int x = 0; x < D / 64; x++) out[x * 64 + lane] = fw_cvt<T>(any ? o[x] / l : 0.0f);
+        } else {
+            const int64_t slot = (((int64_t)b.r * p.tiles + b.tile) * p.kv_heads + b.kvh) * p.splits + b.split;
+            float *part = p.parts + (slot * p.tile_rows + t - b.t0) * (D + 4);
+            for (int x = 0; x < D / 64; x++) part[x * 64 + lane] = o[x];
+            if (lane == 0) {
+                part[D] = m;
+                part[D + 1] = l;
+            }
+        }
+    }
+}
+
 // Few rows (at most 16): the four waves take the chunk's steps of KEYS keys in
 // turn, all with the same rows, and are joined at the end.  Bound by the cache's
 // bytes, so nothing stands between memory and the lanes: a wave's K tile goes
@@ -474,8 +512,7 @@ __global__ void __launch_bounds__(256, 2) k_tree_few(TreeP p) {
     const char *vbase = (const char *)((const T *)p.vc + b.kvh * p.head_stride) + c * 16;
     const int last = b.last;
 
-    auto pass = [&](auto careful) {
-        constexpr bool CAREFUL = decltype(careful)::value;
+    {
         int32_t id[KT];
         u4 kf[KT][NS], vf[KT][NS];
         bool gone[KT]; // no such key
@@ -529,26 +566,22 @@ __global__ void __launch_bounds__(256, 2) k_tree_few(TreeP p) {
             for (int k = 0; k < KT; k++)
 #pragma unroll
                 for (int s = 0; s < NS; s++)
-                    *(u4 *)(vt + (k * 16 + lr) * VROW + s * 64 + c * 16) = CAREFUL ? drop_nonfinite<T>(vf[k][s]) : vf[k][s];
+                    *(u4 *)(vt + (k * 16 + lr) * VROW + s * 64 + c * 16) = vf[k][s];
             wave_fence();
             if (j0 + 4 * KEYS < last) {
                 load(j0 + 4 * KEYS);
                 pages(j0 + 8 * KEYS);
             }
-            uint32_t sees[1] = {0xffffffffu};
-            if (j0 + KEYS > min(b.rq.len, last)) sees[0] = rows.mask(p, b.rq, 0, j0, last, z[0]);
-            rows.weigh(0, z[0], zs);
+            if (j0 + KEYS > min(b.rq.len, last)) rows.mask(p, b.rq, 0, j0, last, z[0]);
+            rows.weigh(z, zs);
             rows.template add<VROW>(vt, z);
-            if constexpr (CAREFUL) rows.add_dropped(p, trow, b.kvh, j0, last, z, sees);
         }
-    };
-    pass(std::false_type{});
-    // Outputs that are not finite may come from values a row does not see (0
-    // times infinity) or from the halves of a weight (infinity less infinity):
-    // then once more, such values row by row.
-    if (__any(rows.odd())) pass(std::true_type{});
+    }
+    if (__syncthreads_or(rows.odd())) { // and the V tiles become the outputs' place
+        tree_slow<T, D>(p, b, lds);
+        return;
+    }
     rows.l[0] = quarters_sum(rows.l[0]);
-    __syncthreads(); // the V tiles become the outputs' place
     rows.join(wave, 4, 0, 16, sm, sl, (float *)lds);
     if (wave == 0) rows.store(p, b.rq, b.r, b.tile, b.split, b.kvh, b.t0, b.total, b.whole);
 }
@@ -581,8 +614,7 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
     const char *vbase = (const char *)((const T *)p.vc + b.kvh * p.head_stride) + piece * 16;
     const int last = b.last;
 
-    auto pass = [&](auto careful) {
-        constexpr bool CAREFUL = decltype(careful)::value;
+    {
         int32_t id[NL];
         u4 kf[NL], vf[NL];
         bool gone[NL]; // no such key
@@ -618,7 +650,7 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
             for (int i = 0; i < NL; i++) {
                 const int key = own + i * (256 / NC);
                 *(u4 *)(at + key * KROW + piece * 16) = kf[i];
-                *(u4 *)(at + TK * KROW + key * VROW + piece * 16) = CAREFUL ? drop_nonfinite<T>(vf[i]) : vf[i];
+                *(u4 *)(at + TK * KROW + key * VROW + piece * 16) = vf[i];
             }
         };
         rows.clear();
@@ -650,20 +682,18 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
                 }
             }
             const int j = j0 + wk * KEYS;
-            uint32_t sees[RT];
+            if (j + KEYS > min(b.rq.len, last))
 #pragma unroll
-            for (int x = 0; x < RT; x++) {
-                sees[x] = 0xffffffffu;
-                if (j + KEYS > min(b.rq.len, last)) sees[x] = rows.mask(p, b.rq, x, j, last, z[x]);
-                rows.weigh(x, z[x], zs);
-            }
+                for (int x = 0; x < RT; x++) rows.mask(p, b.rq, x, j, last, z[x]);
+            rows.weigh(z, zs);
             rows.template add<VROW>(vt, z);
-            if constexpr (CAREFUL) rows.add_dropped(p, trow, b.kvh, j, last, z, sees);
             __syncthreads();
         }
-    };
-    pass(std::false_type{});
-    if (__syncthreads_or(rows.odd())) pass(std::true_type{}); // as in k_tree_few
+    }
+    if (__syncthreads_or(rows.odd())) {
+        tree_slow<T, D>(p, b, lds);
+        return;
+    }
 #pragma unroll
     for (int x = 0; x < RT; x++) rows.l[x] = quarters_sum(rows.l[x]);
     if constexpr (WK > 1) rows.join(wk, WK, wr * RT * 16, WR * RT * 16, sm, sl, (float *)lds);
