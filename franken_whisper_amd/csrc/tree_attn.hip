@@ -167,9 +167,8 @@ __device__ __forceinline__ typename Vec4<T>::type pack4(f4 v) {
                           fw_cvt<T>(v[2]).b | (uint32_t)fw_cvt<T>(v[3]).b << 16);
 }
 
-// Bytes from the start of a K/V head's cache to key j of the request, whose page is id.
-__device__ __forceinline__ uint64_t tree_at(const TreeP &p, uint32_t j, uint32_t id) {
-    const uint32_t t = j - fw_div(j, p.page) * p.page.d;
+// Bytes from the start of a K/V head's cache to token t of page id.
+__device__ __forceinline__ uint64_t tree_at(const TreeP &p, uint32_t t, uint32_t id) {
     return (uint64_t)id * p.page_bytes + (uint64_t)t * p.token_bytes;
 }
 
@@ -249,7 +248,7 @@ struct Rows {
             mx[x] = quarters_max(mx[x]) * zs;
             moves |= mx[x] > m[x] + TREE_SLACK;
         }
-        if (__any(moves)) {
+        if (__builtin_expect(__any(moves), 0)) {
 #pragma unroll
             for (int x = 0; x < RT; x++) {
                 const float mn = mx[x] > m[x] + TREE_SLACK ? mx[x] : m[x];
@@ -446,8 +445,9 @@ __device__ __forceinline__ void tree_slow(const TreeP &p, const TreeBlock &b, ch
             float z = -INFINITY;
             int64_t at = -2; // not seen; -1: no page
             if (yes) {
-                const int32_t id = trow[fw_div((uint32_t)j, p.page)];
-                at = (uint32_t)id < (uint32_t)p.n_pages ? (int64_t)tree_at(p, j, id) : -1;
+                const uint32_t pi = fw_div((uint32_t)j, p.page);
+                const int32_t id = trow[pi];
+                at = (uint32_t)id < (uint32_t)p.n_pages ? (int64_t)tree_at(p, j - pi * p.page.d, id) : -1;
                 z = at < 0 ? __builtin_nanf("") : 0.0f;
                 if (at >= 0)
                     for (int e = 0; e < D; e++) z = fmaf(sq[e], fw_to_f32(((const T *)(kbase + at))[e]), z);
@@ -514,20 +514,23 @@ __global__ void __launch_bounds__(256, 2) k_tree_few(TreeP p) {
 
     {
         int32_t id[KT];
+        uint32_t tok[KT]; // within the page
         u4 kf[KT][NS], vf[KT][NS];
         bool gone[KT]; // no such key
         auto pages = [&](int j) {
 #pragma unroll
             for (int k = 0; k < KT; k++) {
                 const int key = j + k * 16 + lr;
-                id[k] = key < last ? trow[fw_div((uint32_t)key, p.page)] : -1;
+                const uint32_t pi = fw_div((uint32_t)key, p.page);
+                id[k] = key < last ? trow[pi] : -1;
+                tok[k] = key - pi * p.page.d;
             }
         };
-        auto load = [&](int j) {
+        auto load = [&] {
 #pragma unroll
             for (int k = 0; k < KT; k++) {
                 gone[k] = (uint32_t)id[k] >= (uint32_t)p.n_pages;
-                const uint64_t at = gone[k] ? 0 : tree_at(p, j + k * 16 + lr, id[k]);
+                const uint64_t at = gone[k] ? 0 : tree_at(p, tok[k], id[k]);
                 const char *ka = kbase + at, *va = vbase + at;
 #pragma unroll
                 for (int s = 0; s < NS; s++) kf[k][s] = *(const u4 *)(ka + s * 64);
@@ -539,11 +542,11 @@ __global__ void __launch_bounds__(256, 2) k_tree_few(TreeP p) {
         int j0 = b.first + wave * KEYS;
         if (j0 < last) {
             pages(j0);
-            load(j0);
+            load();
             pages(j0 + 4 * KEYS);
         }
         for (; j0 < last; j0 += 4 * KEYS) {
-            if (__any(gone[0] || gone[KT - 1])) {
+            if (__builtin_expect(__any(gone[0] || gone[KT - 1]), 0)) {
 #pragma unroll
                 for (int k = 0; k < KT; k++)
                     if (gone[k])
@@ -569,10 +572,10 @@ __global__ void __launch_bounds__(256, 2) k_tree_few(TreeP p) {
                     *(u4 *)(vt + (k * 16 + lr) * VROW + s * 64 + c * 16) = vf[k][s];
             wave_fence();
             if (j0 + 4 * KEYS < last) {
-                load(j0 + 4 * KEYS);
+                load();
                 pages(j0 + 8 * KEYS);
             }
-            if (j0 + KEYS > min(b.rq.len, last)) rows.mask(p, b.rq, 0, j0, last, z[0]);
+            if (__builtin_expect(j0 + KEYS > min(b.rq.len, last), 0)) rows.mask(p, b.rq, 0, j0, last, z[0]);
             rows.weigh(z, zs);
             rows.template add<VROW>(vt, z);
         }
@@ -616,20 +619,23 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
 
     {
         int32_t id[NL];
+        uint32_t tok[NL]; // within the page
         u4 kf[NL], vf[NL];
         bool gone[NL]; // no such key
         auto pages = [&](int j) {
 #pragma unroll
             for (int i = 0; i < NL; i++) {
                 const int key = j + own + i * (256 / NC);
-                id[i] = key < last ? trow[fw_div((uint32_t)key, p.page)] : -1;
+                const uint32_t pi = fw_div((uint32_t)key, p.page);
+                id[i] = key < last ? trow[pi] : -1;
+                tok[i] = key - pi * p.page.d;
             }
         };
-        auto load = [&](int j) {
+        auto load = [&] {
 #pragma unroll
             for (int i = 0; i < NL; i++) {
                 gone[i] = (uint32_t)id[i] >= (uint32_t)p.n_pages;
-                const uint64_t at = gone[i] ? 0 : tree_at(p, j + own + i * (256 / NC), id[i]);
+                const uint64_t at = gone[i] ? 0 : tree_at(p, tok[i], id[i]);
                 kf[i] = *(const u4 *)(kbase + at);
                 vf[i] = *(const u4 *)(vbase + at);
             }
@@ -638,7 +644,7 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
             bool any = false;
 #pragma unroll
             for (int i = 0; i < NL; i++) any |= gone[i];
-            if (__any(any)) {
+            if (__builtin_expect(__any(any), 0)) {
 #pragma unroll
                 for (int i = 0; i < NL; i++)
                     if (gone[i]) {
@@ -656,16 +662,16 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
         rows.clear();
         int j0 = b.first;
         pages(j0);
-        load(j0);
+        load();
         pages(j0 + TK);
         put(lds);
-        load(j0 + TK);
+        load();
         pages(j0 + 2 * TK);
         __syncthreads();
         for (int at = 0; j0 < last; j0 += TK, at ^= 1) {
             const char *kt = lds + at * TILE + wk * KEYS * KROW, *vt = lds + at * TILE + TK * KROW + wk * KEYS * VROW;
             put(lds + (at ^ 1) * TILE);
-            load(j0 + 2 * TK);
+            load();
             pages(j0 + 3 * TK);
             f4 z[RT][KT];
 #pragma unroll
@@ -682,7 +688,7 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
                 }
             }
             const int j = j0 + wk * KEYS;
-            if (j + KEYS > min(b.rq.len, last))
+            if (__builtin_expect(j + KEYS > min(b.rq.len, last), 0))
 #pragma unroll
                 for (int x = 0; x < RT; x++) rows.mask(p, b.rq, x, j, last, z[x]);
             rows.weigh(z, zs);
