@@ -12,9 +12,8 @@
 #include "fw_paged.h"
 #include "fw_serve.h"
 
-#define TREE_BLOCKS 1024
-#define TREE_CHUNK 512
-#define TREE_ENOUGH 256
+#define TREE_UNITS 1024 // units of a call, at most
+#define TREE_CHUNK 512  // keys of a unit, at least
 
 struct TreeP {
     int n_req, n_rows, heads, kv_heads, n_pages, width, max_new, max_len, words;
@@ -26,9 +25,10 @@ struct TreeP {
     const int32_t *table, *len, *row_start;
     const uint64_t *mask;
     void *out;
-    // how the call is cut (tree_cut): key splits and their length, row tiles and
-    // their rows, the parts [request, tile, K/V head, split, row, D + 4]
-    int splits, chunk, tiles, tile_rows;
+    // how the call is cut (tree_cut): row tiles and their rows; units of keys, or 0
+    // where a block takes all keys of its request; the units' parts [unit, tile, K/V
+    // head, row, D + 4]
+    int tiles, tile_rows, units;
     float *parts;
 };
 
@@ -132,6 +132,51 @@ __device__ __forceinline__ TreeReq tree_req(const TreeP &p, int r) {
     q.len = p.len[r];
     q.bad = q.len < 0 || q.n > p.max_new || (int64_t)q.len + q.n > p.max_len;
     return q;
+}
+// The keys of all requests as units of `chunk` keys, the last of each request
+// shorter: as few keys a unit as keep the units within p.units (a request adds at
+// most one that is not full).  Each wave finds this from the lengths by itself.
+// unit < 0: where request r begins; else the request that holds unit (n_req: none).
+struct TreeUnits {
+    int chunk, r, first, count; // a request, its first unit and how many it has
+};
+__device__ __forceinline__ TreeUnits tree_units(const TreeP &p, int unit, int r) {
+    const int lane = threadIdx.x & 63;
+    auto keys = [&](int i) {
+        if (i >= p.n_req) return 0;
+        const TreeReq q = tree_req(p, i);
+        return q.bad || q.n == 0 ? 0 : q.len + q.n;
+    };
+    int64_t total = 0;
+    for (int i = lane; i < p.n_req; i += 64) total += keys(i);
+    total = fw_wave_sum(total);
+    // fewer than total / chunk + n_req units come of it (the host sees to units > n_req)
+    const int64_t whole = p.units - p.n_req + 1, full = (total + whole - 1) / whole;
+    TreeUnits u;
+    u.chunk = (int)max((full + 127) / 128 * 128, (int64_t)TREE_CHUNK);
+    u.r = p.n_req;
+    u.first = u.count = 0;
+    int before = 0;
+    for (int i0 = 0; i0 < p.n_req; i0 += 64) {
+        const int n = (keys(i0 + lane) + u.chunk - 1) / u.chunk;
+        int sum = n; // of this request and those before it
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int v = __shfl_up(sum, o, 64);
+            if (lane >= o) sum += v;
+        }
+        const bool hit = unit < 0 ? i0 + lane == r : unit < before + sum;
+        const uint64_t who = __ballot(hit);
+        if (who) {
+            const int at = __ffsll((unsigned long long)who) - 1;
+            u.r = i0 + at;
+            u.count = __shfl(n, at, 64);
+            u.first = before + __shfl(sum, at, 64) - u.count;
+            break;
+        }
+        before += __shfl(sum, 63, 64);
+    }
+    return u;
 }
 // Whether new token i of the request sees key j < last.
 __device__ __forceinline__ bool tree_sees(const TreeP &p, const TreeReq &q, int i, int j, int last) {
@@ -354,15 +399,16 @@ struct Rows {
             __syncthreads();
         }
     }
-    // Rows t0 + 0..16 RT - 1 of the tile of R rows that begins at tile0: outputs, or this chunk's part.
-    __device__ __forceinline__ void store(const TreeP &p, const TreeReq &rq, int r, int tile, int split, int kvh, int t0,
-                                          int total, bool whole) {
+    // Rows t0 + 0..16 RT - 1: outputs, or this unit's part.
+    template <typename B>
+    __device__ __forceinline__ void store(const TreeP &p, const B &b, int t0) {
+        const TreeReq &rq = b.rq;
         const int lane = threadIdx.x & 63, lr = lane & 15, c = lane >> 4;
 #pragma unroll
         for (int x = 0; x < RT; x++) {
             const int t = t0 + x * 16 + lr;
-            if (t >= total) continue;
-            if (whole) {
+            if (t >= b.total) continue;
+            if (b.whole) {
                 T *out = (T *)p.out + (int64_t)(rq.row0 + node[x]) * p.out_row + head[x] * p.out_head + 4 * c;
                 const bool any = tree_sees_any(p, rq, node[x]);
                 const float inv = 1.0f / l[x];
@@ -373,8 +419,7 @@ struct Rows {
                     *(typename Vec4<T>::type *)(out + 16 * d) = pack4<T>(v);
                 }
             } else {
-                const int64_t slot = (((int64_t)r * p.tiles + tile) * p.kv_heads + kvh) * p.splits + split;
-                float *at = p.parts + (slot * p.tile_rows + t - tile * p.tile_rows) * (D + 4);
+                float *at = b.part(p, D, t - b.t0);
 #pragma unroll
                 for (int d = 0; d < DT; d++) *(f4 *)(at + 16 * d + 4 * c) = o[x][d];
                 if (c == 0) {
@@ -389,20 +434,28 @@ struct Rows {
 // Where a block stands: its chunk of keys of one K/V head of one request.
 struct TreeBlock {
     TreeReq rq;
-    int r, split, kvh, tile, group, total, t0, first, last;
+    int r, kvh, tile, group, total, t0, first, last;
     bool whole;
     // false: nothing to do (or done: rows of a bad request)
     template <typename T, int D>
     __device__ __forceinline__ bool find(const TreeP &p) {
-        split = blockIdx.x;
-        kvh = blockIdx.y % p.kv_heads;
-        tile = blockIdx.y / p.kv_heads;
-        r = blockIdx.z;
-        rq = tree_req(p, r);
+        kvh = blockIdx.x % p.kv_heads; // heads of a token lie next to each other, their blocks too
+        tile = blockIdx.x / p.kv_heads;
         group = p.heads / p.kv_heads;
-        whole = p.splits == 1;
-        if (rq.bad) { // may have more rows than there are tiles; the join writes them where there is one
-            if (whole && tile == 0)
+        whole = p.units == 0;
+        int chunk = 0;
+        r = blockIdx.y;
+        first = 0;
+        if (!whole) {
+            const TreeUnits u = tree_units(p, blockIdx.y, 0);
+            if (u.r == p.n_req) return false;
+            r = u.r;
+            chunk = u.chunk;
+            first = (blockIdx.y - u.first) * chunk;
+        }
+        rq = tree_req(p, r);
+        if (rq.bad) { // may have more rows than there are tiles (with units the join writes them)
+            if (tile == 0)
                 for (int64_t e = threadIdx.x; e < (int64_t)rq.n * group * D; e += 256) {
                     const int64_t i = e / D / group, h = kvh * group + e / D % group;
                     ((T *)p.out)[(rq.row0 + i) * p.out_row + h * p.out_head + e % D] = fw_cvt<T>(__builtin_nanf(""));
@@ -414,9 +467,12 @@ struct TreeBlock {
         if (t0 >= total) return false;
         // a chain's rows see no further than the tile's last token
         const int end = p.words ? rq.len + rq.n : rq.len + (min(t0 + p.tile_rows, total) - 1) / group + 1;
-        first = split * p.chunk;
-        last = min(end, first + p.chunk);
+        last = whole ? end : min(end, first + chunk);
         return whole || first < end; // the join reads no part behind the end
+    }
+    // Where this block's part of row t0 + i goes.
+    __device__ __forceinline__ float *part(const TreeP &p, int d, int i) const {
+        return p.parts + ((((int64_t)blockIdx.y * p.tiles + tile) * p.kv_heads + kvh) * p.tile_rows + i) * (d + 4);
     }
 };
 
@@ -475,8 +531,7 @@ __device__ __forceinline__ void tree_slow(const TreeP &p, const TreeBlock &b, ch
             const bool any = tree_sees_any(p, b.rq, i);
             for (int x = 0; x < D / 64; x++) out[x * 64 + lane] = fw_cvt<T>(any ? o[x] / l : 0.0f);
         } else {
-            const int64_t slot = (((int64_t)b.r * p.tiles + b.tile) * p.kv_heads + b.kvh) * p.splits + b.split;
-            float *part = p.parts + (slot * p.tile_rows + t - b.t0) * (D + 4);
+            float *part = b.part(p, D, t - b.t0);
             for (int x = 0; x < D / 64; x++) part[x * 64 + lane] = o[x];
             if (lane == 0) {
                 part[D] = m;
@@ -586,7 +641,7 @@ __global__ void __launch_bounds__(256, 2) k_tree_few(TreeP p) {
     }
     rows.l[0] = quarters_sum(rows.l[0]);
     rows.join(wave, 4, 0, 16, sm, sl, (float *)lds);
-    if (wave == 0) rows.store(p, b.rq, b.r, b.tile, b.split, b.kvh, b.t0, b.total, b.whole);
+    if (wave == 0) rows.store(p, b, b.t0);
 }
 
 // More rows: WR waves take RT tiles of rows each, 4 / WR waves the same rows
@@ -703,7 +758,7 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
 #pragma unroll
     for (int x = 0; x < RT; x++) rows.l[x] = quarters_sum(rows.l[x]);
     if constexpr (WK > 1) rows.join(wk, WK, wr * RT * 16, WR * RT * 16, sm, sl, (float *)lds);
-    if (wk == 0) rows.store(p, b.rq, b.r, b.tile, b.split, b.kvh, t0, b.total, b.whole);
+    if (wk == 0) rows.store(p, b, t0);
 }
 
 // The parts of a request's chunks into its outputs: NW waves a row and head.
@@ -712,11 +767,12 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
 template <typename T, int D, int NW>
 __global__ void __launch_bounds__(256) k_tree_join(TreeP p) {
     constexpr int W = D / 4, N = 64 * NW, G = N / W;
-    __shared__ float weight[NW == 1 ? 1 : TREE_BLOCKS], red[8];
+    __shared__ float weight[NW == 1 ? 1 : TREE_UNITS], red[8];
     __shared__ f4 sum[256 / W][W];
     const int r = blockIdx.z, h = blockIdx.y, tid = threadIdx.x % N, own = threadIdx.x / N;
     const TreeReq rq = tree_req(p, r);
     const int group = p.heads / p.kv_heads, kvh = h / group;
+    const TreeUnits un = tree_units(p, -1, r);
     for (int64_t i = (int64_t)blockIdx.x * (256 / N) + own; i < rq.n; i += (int64_t)gridDim.x * (256 / N)) {
         T *out = (T *)p.out + (rq.row0 + i) * p.out_row + (int64_t)h * p.out_head;
         if (rq.bad || !tree_sees_any(p, rq, (int)i)) { // the same for the row's waves
@@ -726,10 +782,9 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeP p) {
         }
         const int t = (int)i * group + h % group, tile = t / p.tile_rows;
         const int keys = rq.len + (p.words ? rq.n : (min((tile + 1) * p.tile_rows, rq.n * group) - 1) / group + 1);
-        const int parts = (keys + p.chunk - 1) / p.chunk; // at most p.splits
-        const int64_t slot = (((int64_t)r * p.tiles + tile) * p.kv_heads + kvh) * p.splits;
-        const float *at = p.parts + (slot * p.tile_rows + t % p.tile_rows) * (D + 4);
-        const int64_t step = (int64_t)p.tile_rows * (D + 4);
+        const int parts = (keys + un.chunk - 1) / un.chunk; // at most un.count
+        const int64_t step = (int64_t)p.tiles * p.kv_heads * p.tile_rows * (D + 4);
+        const float *at = p.parts + un.first * step + (((int64_t)tile * p.kv_heads + kvh) * p.tile_rows + t % p.tile_rows) * (D + 4);
         float mx = -INFINITY, l = 0.0f, mine = -INFINITY;
         if constexpr (NW == 1) {
             if (tid < parts) mine = at[tid * step + D];
@@ -774,11 +829,11 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeP p) {
 }
 
 // How a call of these sizes is cut.  Up to 16 rows per K/V head share one tile
-// (k_tree_few); 32, 64 or 128 rows a block above that (k_tree_wide).  The keys
-// are split until TREE_BLOCKS blocks are there, but not into chunks below
-// TREE_CHUNK keys.
+// (k_tree_few); 32, 64 or 128 rows a block above that (k_tree_wide).  Where that
+// gives fewer than 256 blocks the keys are cut into units (tree_units), as many
+// as run at once: 2 to 4 blocks a CU, by the registers and LDS of the kernel.
 struct TreeCut {
-    int rows, splits, chunk;
+    int rows, units;
     int64_t tiles;
     uint64_t bytes;
 };
@@ -788,28 +843,27 @@ static TreeCut tree_cut(int32_t n_req, int32_t n_heads, int32_t n_kv_heads, int3
     const int64_t rows = (int64_t)max_new * (n_heads / n_kv_heads);
     t.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     t.tiles = (rows + t.rows - 1) / t.rows;
-    const int64_t base = std::max<int64_t>(1, (int64_t)n_req * n_kv_heads * t.tiles);
-    const int64_t most = std::max<int64_t>(1, ((int64_t)max_len + TREE_CHUNK - 1) / TREE_CHUNK);
-    const int64_t blocks = t.rows == 128 ? TREE_BLOCKS / 2 : TREE_BLOCKS;
-    const int64_t want = base >= TREE_ENOUGH ? 1 : std::max<int64_t>(1, std::min(most, blocks / base));
-    t.chunk = (int)((((int64_t)max_len + want - 1) / want + 127) / 128 * 128);
-    t.chunk = std::max(t.chunk, 128);
-    t.splits = (int)std::max<int64_t>(1, ((int64_t)max_len + t.chunk - 1) / t.chunk);
+    const int64_t at_once = head_dim == 64 ? (t.rows == 128 ? 768 : TREE_UNITS) : t.rows == 32 || t.rows == 128 ? 512 : 768;
+    const int64_t per = std::max<int64_t>(1, (int64_t)n_kv_heads * t.tiles), base = per * n_req;
+    const int64_t most = ((int64_t)max_len + TREE_CHUNK - 1) / TREE_CHUNK * n_req; // units of TREE_CHUNK
+    const int64_t units = std::min(at_once / per, most);
+    t.units = base >= 256 || units <= n_req ? 0 : (int)units;
     // enough for every smaller call too
-    t.bytes = most > 1 ? (uint64_t)std::min<int64_t>(TREE_BLOCKS, base * most) * t.rows * (head_dim + 4) * 4 : 0;
+    t.bytes = max_len > TREE_CHUNK ? (uint64_t)std::min(at_once, per * most) * t.rows * (head_dim + 4) * 4 : 0;
     return t;
 }
 
 template <typename T, int D>
 static void tree_go(hipStream_t st, const TreeP &p, int n_req) {
-    const dim3 grid(p.splits, p.kv_heads * p.tiles, n_req), block(256);
+    // without units a block per request
+    const dim3 grid(p.kv_heads * p.tiles, p.units ? p.units : n_req), block(256);
     if (p.tile_rows == 16) hipLaunchKernelGGL((k_tree_few<T, D>), grid, block, 0, st, p);
     else if (p.tile_rows == 32) hipLaunchKernelGGL((k_tree_wide<T, D, 1, 2>), grid, block, 0, st, p);
     else if (p.tile_rows == 64) hipLaunchKernelGGL((k_tree_wide<T, D, 1, 4>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((k_tree_wide<T, D, 2, 4>), grid, block, 0, st, p);
-    if (p.splits == 1) return;
+    if (!p.units) return;
     const unsigned rows = (unsigned)std::min(p.max_new, 4096);
-    if (p.splits <= 64) hipLaunchKernelGGL((k_tree_join<T, D, 1>), dim3((rows + 3) / 4, p.heads, n_req), block, 0, st, p);
+    if (p.units <= 64) hipLaunchKernelGGL((k_tree_join<T, D, 1>), dim3((rows + 3) / 4, p.heads, n_req), block, 0, st, p);
     else hipLaunchKernelGGL((k_tree_join<T, D, 4>), dim3(rows, p.heads, n_req), block, 0, st, p);
 }
 template <typename T>
@@ -903,11 +957,10 @@ extern "C" fwhip_status fwhip_tree_attn(fwhip_ctx *c, const fwhip_tree_attn_args
     p.mask = a->mask;
     p.out = a->out;
     const TreeCut cut = tree_cut(a->n_req, a->n_heads, a->n_kv_heads, a->head_dim, std::min(a->max_new, a->n_rows), a->max_len);
-    if (cut.tiles * a->n_kv_heads > 65535)
-        return fw_fail(FWHIP_ERR_UNSUPPORTED, "fwhip_tree_attn: more than 65535 row tiles x K/V heads");
+    if (cut.tiles * a->n_kv_heads > 1 << 23) // threads of a grid's first dimension stay below 2^32
+        return fw_fail(FWHIP_ERR_UNSUPPORTED, "fwhip_tree_attn: more than 2^23 row tiles x K/V heads");
     p.tiles = (int)cut.tiles;
-    p.splits = cut.splits;
-    p.chunk = cut.chunk;
+    p.units = cut.units;
     p.tile_rows = cut.rows;
     p.parts = (float *)a->workspace;
     if (a->dtype == FWHIP_T_F32) tree_dim<float>(c->stream, a->head_dim, p, a->n_req);
