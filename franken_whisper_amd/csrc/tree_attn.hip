@@ -147,34 +147,35 @@ __device__ __forceinline__ TreeUnits tree_units(const TreeP &p, int unit, int r)
         const TreeReq q = tree_req(p, i);
         return q.bad || q.n == 0 ? 0 : q.len + q.n;
     };
-    int64_t total = 0;
-    for (int i = lane; i < p.n_req; i += 64) total += keys(i);
-    total = fw_wave_sum(total);
+    int mine = keys(lane); // of the first 64 requests
+    double sum = mine;     // exact: whole numbers below 2^53
+    for (int i = lane + 64; i < p.n_req; i += 64) sum += keys(i);
+    const int64_t total = (int64_t)fw_dpp_wave_sum_f64(sum);
     // fewer than total / chunk + n_req units come of it (the host sees to units > n_req)
     const int64_t whole = p.units - p.n_req + 1, full = (total + whole - 1) / whole;
     TreeUnits u;
-    u.chunk = (int)max((full + 127) / 128 * 128, (int64_t)TREE_CHUNK);
+    u.chunk = __builtin_amdgcn_readfirstlane((int)max((full + 127) / 128 * 128, (int64_t)TREE_CHUNK));
     u.r = p.n_req;
     u.first = u.count = 0;
     int before = 0;
     for (int i0 = 0; i0 < p.n_req; i0 += 64) {
-        const int n = (keys(i0 + lane) + u.chunk - 1) / u.chunk;
+        if (i0) mine = keys(i0 + lane);
+        const int n = (mine + u.chunk - 1) / u.chunk;
         int sum = n; // of this request and those before it
 #pragma unroll
         for (int o = 1; o < 64; o *= 2) {
             const int v = __shfl_up(sum, o, 64);
             if (lane >= o) sum += v;
         }
-        const bool hit = unit < 0 ? i0 + lane == r : unit < before + sum;
-        const uint64_t who = __ballot(hit);
-        if (who) {
+        const uint64_t who = __ballot(unit < 0 ? i0 + lane == r : unit < before + sum);
+        if (who) { // the same in every lane, as are all results: they steer the loops
             const int at = __ffsll((unsigned long long)who) - 1;
             u.r = i0 + at;
-            u.count = __shfl(n, at, 64);
-            u.first = before + __shfl(sum, at, 64) - u.count;
+            u.count = __builtin_amdgcn_readlane(n, at);
+            u.first = before + __builtin_amdgcn_readlane(sum, at) - u.count;
             break;
         }
-        before += __shfl(sum, 63, 64);
+        before += __builtin_amdgcn_readlane(sum, 63);
     }
     return u;
 }
@@ -449,9 +450,9 @@ struct TreeBlock {
         if (!whole) {
             const TreeUnits u = tree_units(p, blockIdx.y, 0);
             if (u.r == p.n_req) return false;
-            r = u.r;
+            r = __builtin_amdgcn_readfirstlane(u.r);
             chunk = u.chunk;
-            first = (blockIdx.y - u.first) * chunk;
+            first = __builtin_amdgcn_readfirstlane((blockIdx.y - u.first) * chunk);
         }
         rq = tree_req(p, r);
         if (rq.bad) { // may have more rows than there are tiles (with units the join writes them)
@@ -761,59 +762,56 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
     if (wk == 0) rows.store(p, b, t0);
 }
 
-// The parts of a request's chunks into its outputs: NW waves a row and head.
-// The parts' weights first (a lane each), then the sum, D / 4 lanes a part and
-// 256 NW / D parts at once.  NW = 1 holds the weights in its lanes (at most 64).
+// The parts of a request's units into its outputs: NW waves a row and head.  64
+// parts at a time a lane each finds their weights, then D / 4 lanes a part and
+// 256 NW / D parts at once add them up.  One wave where there are many rows, four
+// where few rows have many parts.
 template <typename T, int D, int NW>
 __global__ void __launch_bounds__(256) k_tree_join(TreeP p) {
-    constexpr int W = D / 4, N = 64 * NW, G = N / W;
-    __shared__ float weight[NW == 1 ? 1 : TREE_UNITS], red[8];
+    constexpr int W = D / 4, N = 64 * NW, G = N / W; // G parts at once
     __shared__ f4 sum[256 / W][W];
-    const int r = blockIdx.z, h = blockIdx.y, tid = threadIdx.x % N, own = threadIdx.x / N;
+    const int r = blockIdx.z, h = blockIdx.y, tid = threadIdx.x % N, own = threadIdx.x / N, lane = threadIdx.x & 63;
     const TreeReq rq = tree_req(p, r);
     const int group = p.heads / p.kv_heads, kvh = h / group;
     const TreeUnits un = tree_units(p, -1, r);
+    const int64_t step = (int64_t)p.tiles * p.kv_heads * p.tile_rows * (D + 4);
     for (int64_t i = (int64_t)blockIdx.x * (256 / N) + own; i < rq.n; i += (int64_t)gridDim.x * (256 / N)) {
         T *out = (T *)p.out + (rq.row0 + i) * p.out_row + (int64_t)h * p.out_head;
-        if (rq.bad || !tree_sees_any(p, rq, (int)i)) { // the same for the row's waves
-            const float v = rq.bad ? __builtin_nanf("") : 0.0f;
-            if (tid < W) *(typename Vec4<T>::type *)(out + 4 * tid) = pack4<T>(f4{v, v, v, v});
+        if (rq.bad) {
+            if (tid < W) *(typename Vec4<T>::type *)(out + 4 * tid) = pack4<T>(f4{} + __builtin_nanf(""));
             continue;
         }
+        const bool any = tree_sees_any(p, rq, (int)i);
         const int t = (int)i * group + h % group, tile = t / p.tile_rows;
         const int keys = rq.len + (p.words ? rq.n : (min((tile + 1) * p.tile_rows, rq.n * group) - 1) / group + 1);
         const int parts = (keys + un.chunk - 1) / un.chunk; // at most un.count
-        const int64_t step = (int64_t)p.tiles * p.kv_heads * p.tile_rows * (D + 4);
         const float *at = p.parts + un.first * step + (((int64_t)tile * p.kv_heads + kvh) * p.tile_rows + t % p.tile_rows) * (D + 4);
-        float mx = -INFINITY, l = 0.0f, mine = -INFINITY;
-        if constexpr (NW == 1) {
-            if (tid < parts) mine = at[tid * step + D];
-            mx = fw_wave_max(mine);
-            mine = __builtin_amdgcn_exp2f(mine - TREE_BIAS - tree_base(mx));
-            if (tid < parts) l = mine * at[tid * step + D + 1];
-            l = fw_wave_sum(l);
-        } else {
-            __syncthreads();
-            for (int s = tid; s < parts; s += N) mx = fmaxf(mx, weight[s] = at[s * step + D]);
-            mx = fw_block_max(mx, red);
-            for (int s = tid; s < parts; s += N) {
-                const float f = __builtin_amdgcn_exp2f(weight[s] - TREE_BIAS - tree_base(mx));
-                weight[s] = f;
-                l = fmaf(f, at[s * step + D + 1], l);
-            }
-            l = fw_block_sum(l, red);
-        }
+        float mx = -INFINITY;
+        for (int s = lane; s < parts; s += 64) mx = fmaxf(mx, at[s * step + D]);
+        mx = fw_dpp_wave_max(mx);
+        const float base = tree_base(mx);
+        float l = 0.0f;
         f4 o = {};
+        for (int s0 = 0; s0 < parts; s0 += 64) {
+            float mine = 0.0f;
+            if (s0 + lane < parts) {
+                const float2 ml = *(const float2 *)(at + (s0 + lane) * step + D);
+                mine = __builtin_amdgcn_exp2f(ml.x - TREE_BIAS - base);
+                l = fmaf(mine, ml.y, l);
+            }
+            const int n = min(parts - s0, 64);
 #pragma unroll 4
-        for (int s0 = 0; s0 < parts; s0 += G) { // the same turns for every lane: the exchange needs them all
-            const int s = s0 + tid / W;
-            const float f = NW == 1 ? __shfl(mine, s) : weight[min(s, parts - 1)];
-            if (s < parts) {
-                const f4 v = *(const f4 *)(at + s * step + 4 * (tid % W));
+            for (int k = 0; k < n; k += G) { // the same turns for every lane: the exchange needs them all
+                const int s = k + tid / W;
+                const float f = __shfl(mine, s & 63);
+                if (s < n) {
+                    const f4 v = *(const f4 *)(at + (s0 + s) * step + 4 * (tid % W));
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[e] = fmaf(f, v[e], o[e]);
+                    for (int e = 0; e < 4; e++) o[e] = fmaf(f, v[e], o[e]);
+                }
             }
         }
+        l = fw_wave_sum(l);
         f4 *all = &sum[own * G][0];
         all[tid] = o;
         if constexpr (NW == 1) wave_fence();
@@ -822,9 +820,11 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeP p) {
 #pragma unroll
             for (int g = 1; g < G; g++) o += all[g * W + tid];
             const float inv = 1.0f / l;
-            *(typename Vec4<T>::type *)(out + 4 * tid) = pack4<T>(l == 0.0f ? f4{} + __builtin_nanf("") : o * inv);
+            const f4 v = l == 0.0f ? f4{} + __builtin_nanf("") : o * inv; // 0 / 0: every key scored -inf
+            *(typename Vec4<T>::type *)(out + 4 * tid) = pack4<T>(any ? v : f4{});
         }
         if constexpr (NW == 1) wave_fence();
+        else __syncthreads();
     }
 }
 
@@ -862,9 +862,12 @@ static void tree_go(hipStream_t st, const TreeP &p, int n_req) {
     else if (p.tile_rows == 64) hipLaunchKernelGGL((k_tree_wide<T, D, 1, 4>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((k_tree_wide<T, D, 2, 4>), grid, block, 0, st, p);
     if (!p.units) return;
-    const unsigned rows = (unsigned)std::min(p.max_new, 4096);
-    if (p.units <= 64) hipLaunchKernelGGL((k_tree_join<T, D, 1>), dim3((rows + 3) / 4, p.heads, n_req), block, 0, st, p);
-    else hipLaunchKernelGGL((k_tree_join<T, D, 4>), dim3(rows, p.heads, n_req), block, 0, st, p);
+    // about four blocks a CU, each going through several rows where there are more
+    const bool one = (int64_t)p.max_new * p.heads * n_req >= 1024;
+    const int64_t rows = one ? ((int64_t)p.max_new + 3) / 4 : p.max_new, most = std::max(1, 1024 / std::max(1, p.heads * n_req));
+    const dim3 jgrid((unsigned)std::max<int64_t>(1, std::min(rows, most)), p.heads, n_req);
+    if (one) hipLaunchKernelGGL((k_tree_join<T, D, 1>), jgrid, block, 0, st, p);
+    else hipLaunchKernelGGL((k_tree_join<T, D, 4>), jgrid, block, 0, st, p);
 }
 template <typename T>
 static void tree_dim(hipStream_t st, int d, const TreeP &p, int n_req) {
