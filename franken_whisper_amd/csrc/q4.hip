@@ -19,7 +19,7 @@ struct Q4P {
     const float *bias;
     void *y;
     int scale32, vec, pair; // planes of f32; x rows 16-byte (f32) or 8-byte aligned; four f16 scales so aligned
-    int chunk, lds;          // inputs staged at a time; bytes of LDS
+    int chunk, stage, lds;   // inputs staged at a time; bytes of a stage, and of LDS in all
 };
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -138,11 +138,11 @@ __device__ __forceinline__ float q4_one(const Q4P &p, int m, int n) {
 
 // The kernel: MT * 16 rows of x by WN waves of NT * 16 outputs each, WK waves
 // taking turns of MS steps of the same outputs.  x is staged in LDS for up to
-// `chunk` inputs at a time, its sums beside it where weights have a minimum;
-// each wave streams its weights straight to registers, one turn ahead.  GB: the
+// `chunk` inputs at a time, its sums beside it where weights have a minimum (all
+// of x where it fits, else in two stages that take turns); each wave streams its weights straight to registers, one turn ahead.  GB: the
 // 32-weight blocks of a group.  Of a turn's 4 MS blocks a lane quarter loads the
 // scales of its MS, which the quarters then exchange.
-template <typename T, bool MIN, int GB, int MT, int NT, int WN, int WK, int MS>
+template <typename T, bool MIN, int GB, int MT, int NT, int WN, int WK, int MS, bool TWO>
 __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
     constexpr bool BF = std::is_same<T, fw_bf16>::value, F32 = std::is_same<T, float>::value, CORR = MIN || BF;
     constexpr int PARTS = Q4X<T>::PARTS, NW = WN * WK, R = MT * 16;
@@ -156,10 +156,8 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
     const int cturns = p.chunk / (128 * MS), turns = (p.k + 128 * MS - 1) / (128 * MS);
     const int xrow = p.chunk * 2 + 16; // bytes of a row: rows 4 banks apart
     const int plane = rows * xrow;
-    int *odd = (int *)lds;                                      // [R]: rows with a value that is not finite
-    char *xt = lds + R * 4;                                     // x: [part][row][xrow]
-    float *sums = (float *)(xt + PARTS * plane);                // CORR: [turn][MS][4][R], see below
-    float *scal = sums + (CORR ? cturns * MS * 4 * R : 0);      // f32: [turn][R]
+    int *odd = (int *)lds;    // [R]: rows with a value that is not finite
+    char *stage0 = lds + R * 4; // one or two stages: x [part][row][xrow], CORR: sums [turn][MS][4][R], f32: scales [turn][R]
     Q4Magic magic = BF ? Q4Magic{0x43004300u, 0} : Q4Magic{0x64006400u, 0x54005400u};
     asm volatile("" : "+v"(magic.lo), "+v"(magic.hi));
 
@@ -218,93 +216,114 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
     };
     auto value = [&](uint32_t v) { return p.scale32 ? __uint_as_float(v) : fw_to_f32(fw_f16{(uint16_t)v}); };
 
-    for (int t0 = 0; t0 < turns; t0 += cturns) {
-        const int to = min(turns, t0 + cturns);
-        if (t0 + wk < to) load(t0 + wk);
-        if (t0) __syncthreads();
-        // stage x: a unit of 8 inputs per lane, 16 MS of them a row's turn; four
-        // row's turns are on their way from memory at once
-        constexpr int UN = 16 * MS, PER = NW * 64 / UN, AT = 4;
-        const int items = rows * (to - t0), u = lane % UN;
-        const float per_row = 1.0f / (float)rows; // (i + 1/2) / rows, cut, is i / rows: items stay below 2^16
-        for (int i0 = threadIdx.x / UN; i0 < items; i0 += AT * PER) {
-            Q4Four<T> xe[AT], xh[AT];
-            int row[AT], turn[AT];
+    // staging x: a unit of 8 inputs per lane, 16 MS of them a row's turn; AT rows'
+    // turns a lane are on their way from memory at once
+    constexpr int UN = 16 * MS, PER = NW * 64 / UN;
+    // fewer where their registers would be missed: f32 fetches are twice as wide, and
+    // 8 tiles with a scale a block fill the file
+    constexpr int AT = F32 ? 2 : MT * NT >= 8 && GB == 1 ? 1 : 4;
+    const float per_row = 1.0f / (float)rows; // (i + 1/2) / rows, cut, is i / rows: items stay below 2^16
+    const int u = lane % UN;
+    Q4Four<T> xe[AT], xh[AT];
+    auto fetch = [&](int t0, int to, int i0) { // items i0 + j * PER of the turns t0 .. to - 1
+        const int items = rows * (to - t0);
 #pragma unroll
-            for (int j = 0; j < AT; j++) {
-                const int it = min(i0 + j * PER, items - 1);
-                turn[j] = (int)(((float)it + 0.5f) * per_row);
-                row[j] = it - turn[j] * rows;
-                const int blk = min((t0 + turn[j]) * 4 * MS + (u >> 2), blocks - 1);
-                const T *at = (const T *)p.x + (int64_t)(m0 + row[j]) * p.ldx + (blk * 32 + (u & 3) * 4);
-                xe[j].load(at, p.vec);
-                xh[j].load(at + 16, p.vec);
+        for (int j = 0; j < AT; j++) {
+            const int it = min(i0 + j * PER, items - 1), t = (int)(((float)it + 0.5f) * per_row), r = it - t * rows;
+            const int blk = min((t0 + t) * 4 * MS + (u >> 2), blocks - 1);
+            const T *at = (const T *)p.x + (int64_t)(m0 + r) * p.ldx + (blk * 32 + (u & 3) * 4);
+            xe[j].load(at, p.vec);
+            xh[j].load(at + 16, p.vec);
+        }
+    };
+    auto put = [&](int t0, int to, int i0, char *xt) {
+        const int items = rows * (to - t0);
+        float *sums = (float *)(xt + PARTS * plane), *scal = sums + (CORR ? cturns * MS * 4 * R : 0);
+#pragma unroll
+        for (int j = 0; j < AT; j++) {
+            const int it = i0 + j * PER, t = (int)(((float)it + 0.5f) * per_row), r = it - t * rows;
+            if (it < items) {
+            if ((t0 + t) * 4 * MS + (u >> 2) >= blocks) {
+                xe[j].clear();
+                xh[j].clear();
             }
+            if constexpr (CORR) {
+                // sums of the inputs of each group (or part of one, where it is longer than a quarter)
+                float v = xh[j].sum(xe[j].sum(0.0f));
+                v = v + fw_dpp_f32<FW_DPP_XOR1>(v);
+                v = v + fw_dpp_f32<FW_DPP_XOR2>(v);
+                if (!(fabsf(v) < INFINITY)) odd[r] = 1;
+                if constexpr (GB >= 2 && MS >= 2) v = v + fw_dpp_f32<FW_DPP_HALF_MIRROR>(v);
+                if constexpr (GB >= 4 && MS >= 4) v = v + fw_dpp_f32<FW_DPP_MIRROR>(v);
+                // block b of the turn: quarter b / MS, its scale (b % MS) / GB
+                const int b = u >> 2;
+                if ((u & 3) == 0 && b % MS % GB == 0) sums[((t * MS + b % MS / GB) * 4 + b / MS) * R + r] = v;
+            }
+            char *to_lds = xt + r * xrow + t * (256 * MS) + u * 16;
+            if constexpr (F32) {
+                float e[4], h[4], el[4], hl[4], mx = 0.0f;
 #pragma unroll
-            for (int j = 0; j < AT; j++) {
-                if (i0 + j * PER >= items) break;
-                const int r = row[j], t = turn[j];
-                if ((t0 + t) * 4 * MS + (u >> 2) >= blocks) {
-                    xe[j].clear();
-                    xh[j].clear();
+                for (int i = 0; i < 4; i++) {
+                    e[i] = __uint_as_float(xe[j].v[i]);
+                    h[i] = __uint_as_float(xh[j].v[i]);
+                    mx = fmaxf(mx, fabsf(e[i]) < INFINITY ? fabsf(e[i]) : 0.0f);
+                    mx = fmaxf(mx, fabsf(h[i]) < INFINITY ? fabsf(h[i]) : 0.0f);
                 }
-                if constexpr (CORR) {
-                    // sums of the inputs of each group (or part of one, where it is longer than a quarter)
-                    float v = xh[j].sum(xe[j].sum(0.0f));
-                    v = v + fw_dpp_f32<FW_DPP_XOR1>(v);
-                    v = v + fw_dpp_f32<FW_DPP_XOR2>(v);
-                    if (!(fabsf(v) < INFINITY)) odd[r] = 1;
-                    if constexpr (GB >= 2 && MS >= 2) v = v + fw_dpp_f32<FW_DPP_HALF_MIRROR>(v);
-                    if constexpr (GB >= 4 && MS >= 4) v = v + fw_dpp_f32<FW_DPP_MIRROR>(v);
-                    // block b of the turn: quarter b / MS, its scale (b % MS) / GB
-                    const int b = u >> 2;
-                    if ((u & 3) == 0 && b % MS % GB == 0) sums[((t * MS + b % MS / GB) * 4 + b / MS) * R + r] = v;
+                mx = fmaxf(mx, fw_dpp_f32<FW_DPP_XOR1>(mx));
+                mx = fmaxf(mx, fw_dpp_f32<FW_DPP_XOR2>(mx));
+                mx = fmaxf(mx, fw_dpp_f32<FW_DPP_HALF_MIRROR>(mx));
+                mx = fmaxf(mx, fw_dpp_f32<FW_DPP_MIRROR>(mx));
+#pragma unroll
+                for (int o = 16; o < UN; o *= 2) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+                // mx = 1.f x 2^(ex - 127); x is scaled by 2^(14 - (ex - 127)), in two factors that are normal numbers
+                const int ex = max((int)(__float_as_uint(mx) >> 23), 1), up = 141 - ex;
+                const float f1 = __uint_as_float((uint32_t)(127 + up / 2) << 23), f2 = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    e[i] = e[i] * f1 * f2;
+                    h[i] = h[i] * f1 * f2;
+                    // second parts; of values that are not finite: nothing more
+                    el[i] = fabsf(e[i]) < INFINITY ? e[i] - (float)(_Float16)e[i] : 0.0f;
+                    hl[i] = fabsf(h[i]) < INFINITY ? h[i] - (float)(_Float16)h[i] : 0.0f;
                 }
-                char *to_lds = xt + r * xrow + t * (256 * MS) + u * 16;
-                if constexpr (F32) {
-                    float e[4], h[4], el[4], hl[4], mx = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        e[i] = __uint_as_float(xe[j].v[i]);
-                        h[i] = __uint_as_float(xh[j].v[i]);
-                        mx = fmaxf(mx, fabsf(e[i]) < INFINITY ? fabsf(e[i]) : 0.0f);
-                        mx = fmaxf(mx, fabsf(h[i]) < INFINITY ? fabsf(h[i]) : 0.0f);
-                    }
-                    mx = fmaxf(mx, fw_dpp_f32<FW_DPP_XOR1>(mx));
-                    mx = fmaxf(mx, fw_dpp_f32<FW_DPP_XOR2>(mx));
-                    mx = fmaxf(mx, fw_dpp_f32<FW_DPP_HALF_MIRROR>(mx));
-                    mx = fmaxf(mx, fw_dpp_f32<FW_DPP_MIRROR>(mx));
-#pragma unroll
-                    for (int o = 16; o < UN; o *= 2) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-                    // mx = 1.f x 2^(ex - 127); x is scaled by 2^(14 - (ex - 127)), in two factors that are normal numbers
-                    const int ex = max((int)(__float_as_uint(mx) >> 23), 1), up = 141 - ex;
-                    const float f1 = __uint_as_float((uint32_t)(127 + up / 2) << 23), f2 = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        e[i] = e[i] * f1 * f2;
-                        h[i] = h[i] * f1 * f2;
-                        // second parts; of values that are not finite: nothing more
-                        el[i] = fabsf(e[i]) < INFINITY ? e[i] - (float)(_Float16)e[i] : 0.0f;
-                        hl[i] = fabsf(h[i]) < INFINITY ? h[i] - (float)(_Float16)h[i] : 0.0f;
-                    }
-                    // up is -113..140: the inverse 2^-up as a number, subnormal ones included
-                    if (u == 0) scal[t * R + r] = __builtin_ldexpf(1.0f, -up);
-                    *(u4 *)to_lds = u4{q4_pair(e[0], e[2]), q4_pair(h[0], h[2]), q4_pair(e[1], e[3]), q4_pair(h[1], h[3])};
-                    *(u4 *)(to_lds + plane) = u4{q4_pair(el[0], el[2]), q4_pair(hl[0], hl[2]), q4_pair(el[1], el[3]), q4_pair(hl[1], hl[3])};
-                } else {
-                    const uint2 e = xe[j].v, h = xh[j].v;
-                    *(u4 *)to_lds = u4{__builtin_amdgcn_perm(e.y, e.x, 0x05040100), __builtin_amdgcn_perm(h.y, h.x, 0x05040100),
-                                       __builtin_amdgcn_perm(e.y, e.x, 0x07060302), __builtin_amdgcn_perm(h.y, h.x, 0x07060302)};
-                }
+                // up is -113..140: the inverse 2^-up as a number, subnormal ones included
+                if (u == 0) scal[t * R + r] = __builtin_ldexpf(1.0f, -up);
+                *(u4 *)to_lds = u4{q4_pair(e[0], e[2]), q4_pair(h[0], h[2]), q4_pair(e[1], e[3]), q4_pair(h[1], h[3])};
+                *(u4 *)(to_lds + plane) = u4{q4_pair(el[0], el[2]), q4_pair(hl[0], hl[2]), q4_pair(el[1], el[3]), q4_pair(hl[1], hl[3])};
+            } else {
+                const uint2 e = xe[j].v, h = xh[j].v;
+                *(u4 *)to_lds = u4{__builtin_amdgcn_perm(e.y, e.x, 0x05040100), __builtin_amdgcn_perm(h.y, h.x, 0x05040100),
+                                   __builtin_amdgcn_perm(e.y, e.x, 0x07060302), __builtin_amdgcn_perm(h.y, h.x, 0x07060302)};
+            }
             }
         }
-        __syncthreads();
+    };
+
+    const int stage_bytes = p.stage, item0 = threadIdx.x / UN;
+    // the items of a stage: the first batch is fetched already, the others (if any) here
+    auto fill = [&](int t0, int to, char *xt) {
+        put(t0, to, item0, xt);
+        for (int i0 = item0 + AT * PER; i0 < rows * (to - t0); i0 += AT * PER) {
+            fetch(t0, to, i0);
+            put(t0, to, i0, xt);
+        }
+    };
+    if (wk < turns) load(wk);
+    fetch(0, min(turns, cturns), item0);
+    fill(0, min(turns, cturns), stage0);
+    if (cturns < turns) fetch(cturns, min(turns, 2 * cturns), item0);
+    __syncthreads();
+    int mine = wk; // this wave's next turn
+    for (int t0 = 0, at = 0; t0 < turns; t0 += cturns, at ^= 1) {
+        const int to = min(turns, t0 + cturns);
+        const char *xt = stage0 + (TWO ? at * stage_bytes : 0);
+        const float *sums = (const float *)(xt + PARTS * plane), *scal = sums + (CORR ? cturns * MS * 4 * R : 0);
 
         const char *xl[MT]; // this lane's units of each row tile (the last row again behind the end)
 #pragma unroll
         for (int x = 0; x < MT; x++) xl[x] = xt + min(x * 16 + lr, rows - 1) * xrow + c * 16;
-        for (int t = t0 + wk; t < to; t += WK) {
-            const int tl = t - t0;
+        for (; mine < to; mine += WK) {
+            const int t = mine, tl = t - t0;
             u4 w[MS][NT];
             float d[SP][NT];
 #pragma unroll
@@ -326,7 +345,7 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
                     }
                 }
             }
-            if (t + WK < to) load(t + WK);
+            if (t + WK < turns) load(t + WK);
             f4 dq[SP][NT];
 #pragma unroll
             for (int y = 0; y < NT; y++)
@@ -388,12 +407,19 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
                 }
             }
         }
+        if (to < turns) {
+            const int t1 = min(turns, to + cturns), t2 = min(turns, t1 + cturns);
+            if (!TWO) __syncthreads(); // the one stage is being read
+            fill(to, t1, stage0 + (TWO ? (at ^ 1) * stage_bytes : 0));
+            if (t1 < turns) fetch(t1, t2, item0);
+            __syncthreads();
+        }
     }
 
     // the waves that shared outputs add up, in order
     if constexpr (WK > 1) {
         __syncthreads();
-        f4 *part = (f4 *)xt; // [wave][x][y][lane]
+        f4 *part = (f4 *)stage0; // [wave][x][y][lane]
         if (wk)
 #pragma unroll
             for (int x = 0; x < MT; x++)
@@ -427,25 +453,33 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
     }
 }
 
-template <typename T, bool MIN, int GB, int MT, int NT, int WN, int WK, int MS>
+template <typename T, bool MIN, int GB, int MT, int NT, int WN, int WK, int MS, bool TWO>
 static void q4_go(hipStream_t st, Q4P p) {
     constexpr bool CORR = MIN || std::is_same<T, fw_bf16>::value, F32 = std::is_same<T, float>::value;
     const int rows = std::min(p.m, MT * 16);
-    // as many inputs a stage as fit 64 KiB of LDS, a whole number of turns of every wave
+    // All of x in one stage where it fits 64 KiB of LDS; else TWO stages, of whole
+    // rounds of the waves' turns in 80 KiB together (two blocks a CU) where one
+    // fits, of as many turns as 144 KiB hold where not; or one of 64 KiB that is
+    // filled again.
     const int turn = MS * (Q4X<T>::PARTS * rows * 256 + (CORR ? 256 * MT : 0)) + (F32 ? 64 * MT : 0);
-    const int fixed = Q4X<T>::PARTS * rows * 16 + 64 * MT, join = 64 * MT + (WK > 1 ? WN * WK * MT * NT * 1024 : 0);
-    int turns = std::max(1, (65536 - fixed) / turn);
-    turns = std::min(turns, (p.k + 128 * MS - 1) / (128 * MS));
-    if (turns > WK) turns = turns / WK * WK;
+    const int fixed = Q4X<T>::PARTS * rows * 16, join = WK > 1 ? WN * WK * MT * NT * 1024 : 0;
+    const int all_turns = (p.k + 128 * MS - 1) / (128 * MS);
+    int turns = all_turns, stages = 1;
+    if (turns * (int64_t)turn + fixed > 65536) {
+        stages = TWO ? 2 : 1;
+        turns = ((TWO ? 40960 : 65536) - fixed) / turn / WK * WK;
+        if (turns < 1) turns = std::max(1, std::min(WK, (73728 - fixed) / turn));
+    }
     p.chunk = turns * MS * 128;
-    p.lds = std::max(turns * turn + fixed, join);
+    p.stage = turns * turn + fixed;
+    p.lds = 64 * MT + std::max(stages * p.stage, join);
     const Q4P all = p;
     for (int64_t at = 0; at < all.m; at += 65535 * 16 * MT) { // the grid's reach in rows
         p.m = (int)std::min<int64_t>(all.m - at, 65535 * 16 * MT);
         p.x = (const T *)all.x + at * all.ldx;
         p.y = (T *)all.y + at * all.ldy;
         const dim3 grid((unsigned)((p.n + 16 * NT * WN - 1) / (16 * NT * WN)), (unsigned)((p.m + 16 * MT - 1) / (16 * MT)));
-        hipLaunchKernelGGL((k_q4<T, MIN, GB, MT, NT, WN, WK, MS>), grid, dim3(64 * WN * WK), p.lds, st, p);
+        hipLaunchKernelGGL((k_q4<T, MIN, GB, MT, NT, WN, WK, MS, TWO>), grid, dim3(64 * WN * WK), p.lds, st, p);
     }
 }
 // Which form runs.  x is staged once a block, so many outputs a block save
@@ -463,18 +497,18 @@ template <typename T, bool MIN, int GB>
 static void q4_rows(hipStream_t st, const Q4P &p) {
     const int64_t tiles = (p.n + 15) / 16, mt = (p.m + 63) / 64;
     if (p.m <= 16) {
-        if (tiles <= 640) q4_go<T, MIN, GB, 1, 1, 1, 8, 1>(st, p);
-        else if (p.k < 2048) q4_go<T, MIN, GB, 1, 1, 8, 1, 2>(st, p);
-        else if (tiles <= 1280) q4_go<T, MIN, GB, 1, 1, 4, 2, 4>(st, p);
-        else q4_go<T, MIN, GB, 1, 1, 8, 1, 4>(st, p);
+        if (tiles <= 640) q4_go<T, MIN, GB, 1, 1, 1, 8, 1, true>(st, p);
+        else if (p.k < 2048) q4_go<T, MIN, GB, 1, 1, 8, 1, 2, true>(st, p);
+        else if (tiles <= 1280) q4_go<T, MIN, GB, 1, 1, 4, 2, 4, true>(st, p);
+        else q4_go<T, MIN, GB, 1, 1, 8, 1, 4, true>(st, p);
     } else if (p.m <= 32) {
-        if (tiles <= 128) q4_go<T, MIN, GB, 2, 1, 1, 8, 1>(st, p);
-        else if (tiles <= 512) q4_go<T, MIN, GB, 2, 1, 2, 4, 1>(st, p);
-        else q4_go<T, MIN, GB, 2, 1, 8, 1, 2>(st, p);
-    } else if ((tiles + 15) / 16 * mt >= 256) q4_go<T, MIN, GB, 4, 2, 8, 1, 1>(st, p);
-    else if ((tiles + 7) / 8 * mt >= 128) q4_go<T, MIN, GB, 4, 1, 8, 1, 2>(st, p);
-    else if ((tiles + 3) / 4 * mt >= 96) q4_go<T, MIN, GB, 4, 1, 4, 2, 2>(st, p);
-    else q4_go<T, MIN, GB, 4, 1, 2, 4, 1>(st, p);
+        if (tiles <= 128) q4_go<T, MIN, GB, 2, 1, 1, 8, 1, true>(st, p);
+        else if (tiles <= 512) q4_go<T, MIN, GB, 2, 1, 2, 4, 1, true>(st, p);
+        else q4_go<T, MIN, GB, 2, 1, 8, 1, 2, true>(st, p);
+    } else if ((tiles + 15) / 16 * mt >= 256) q4_go<T, MIN, GB, 4, 2, 8, 1, 1, true>(st, p);
+    else if ((tiles + 7) / 8 * mt >= 128) q4_go<T, MIN, GB, 4, 1, 8, 1, 2, true>(st, p);
+    else if ((tiles + 3) / 4 * mt >= 96) q4_go<T, MIN, GB, 4, 1, 4, 2, 2, true>(st, p);
+    else q4_go<T, MIN, GB, 4, 1, 2, 4, 1, true>(st, p);
 }
 template <typename T>
 static void q4_type(hipStream_t st, const Q4P &p) {
@@ -518,7 +552,7 @@ extern "C" fwhip_status fwhip_q4_linear(fwhip_ctx *c, const fwhip_q4_linear_args
     const int vec = fw_aligned(a->x, vb) && (a->m == 1 || a->ldx * eb % vb == 0);
     const int pair = fw_aligned(a->scale, 8) && fw_aligned(a->minimum, 8) && a->k / a->group % 4 == 0;
     const Q4P p = {a->m, a->n, a->k, a->group, a->ldx, a->ldy, a->x, a->q, a->scale, a->minimum, a->bias, a->y,
-                   a->scale_dtype == FWHIP_T_F32, vec, pair, 0, 0};
+                   a->scale_dtype == FWHIP_T_F32, vec, pair, 0, 0, 0};
     if (a->dtype == FWHIP_T_F32) q4_type<float>(c->stream, p);
     else if (a->dtype == FWHIP_T_F16) q4_type<fw_f16>(c->stream, p);
     else q4_type<fw_bf16>(c->stream, p);
