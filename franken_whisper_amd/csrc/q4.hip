@@ -222,28 +222,43 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
     // fewer where their registers would be missed: f32 fetches are twice as wide, and
     // 8 tiles with a scale a block fill the file
     constexpr int AT = F32 ? 2 : MT * NT >= 8 && GB == 1 ? 1 : 4;
+    const int u = lane % UN, item0 = threadIdx.x / UN;
     const float per_row = 1.0f / (float)rows; // (i + 1/2) / rows, cut, is i / rows: items stay below 2^16
-    const int u = lane % UN;
+    // A lane's items of a batch: row and turn within the stage, where their inputs
+    // begin in memory and their units in LDS.  The first batch is the same in every
+    // stage but for the turns before it, so this is found once.
+    struct Items {
+        int r[AT], t[AT];
+        const T *from[AT];
+    };
     Q4Four<T> xe[AT], xh[AT];
-    auto fetch = [&](int t0, int to, int i0) { // items i0 + j * PER of the turns t0 .. to - 1
-        const int items = rows * (to - t0);
+    auto items = [&](int i0, int n) {
+        Items w;
 #pragma unroll
         for (int j = 0; j < AT; j++) {
-            const int it = min(i0 + j * PER, items - 1), t = (int)(((float)it + 0.5f) * per_row), r = it - t * rows;
-            const int blk = min((t0 + t) * 4 * MS + (u >> 2), blocks - 1);
-            const T *at = (const T *)p.x + (int64_t)(m0 + r) * p.ldx + (blk * 32 + (u & 3) * 4);
+            const int it = i0 + j * PER;
+            w.t[j] = it < n ? (int)(((float)it + 0.5f) * per_row) : 1 << 20; // none: behind the last turn
+            w.r[j] = it < n ? it - w.t[j] * rows : 0;
+            w.from[j] = (const T *)p.x + (int64_t)(m0 + w.r[j]) * p.ldx + (it < n ? (int64_t)w.t[j] * (128 * MS) : 0) + ((u >> 2) * 32 + (u & 3) * 4);
+        }
+        return w;
+    };
+    auto inside = [&](const Items &w, int t0, int j) { return (t0 + w.t[j]) * 4 * MS + (u >> 2) < blocks; };
+    auto fetch = [&](const Items &w, int t0) {
+#pragma unroll
+        for (int j = 0; j < AT; j++) {
+            const T *at = inside(w, t0, j) ? w.from[j] + (int64_t)t0 * (128 * MS) : (const T *)p.x;
             xe[j].load(at, p.vec);
             xh[j].load(at + 16, p.vec);
         }
     };
-    auto put = [&](int t0, int to, int i0, char *xt) {
-        const int items = rows * (to - t0);
+    auto put = [&](const Items &w, int t0, int to, char *xt) {
         float *sums = (float *)(xt + PARTS * plane), *scal = sums + (CORR ? cturns * MS * 4 * R : 0);
 #pragma unroll
         for (int j = 0; j < AT; j++) {
-            const int it = i0 + j * PER, t = (int)(((float)it + 0.5f) * per_row), r = it - t * rows;
-            if (it < items) {
-            if ((t0 + t) * 4 * MS + (u >> 2) >= blocks) {
+            const int t = w.t[j], r = w.r[j];
+            if (t < to - t0) {
+            if (!inside(w, t0, j)) {
                 xe[j].clear();
                 xh[j].clear();
             }
@@ -299,19 +314,21 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
         }
     };
 
-    const int stage_bytes = p.stage, item0 = threadIdx.x / UN;
+    const int stage_bytes = p.stage, full = rows * min(turns, cturns);
+    const Items first = items(item0, full);
     // the items of a stage: the first batch is fetched already, the others (if any) here
     auto fill = [&](int t0, int to, char *xt) {
-        put(t0, to, item0, xt);
-        for (int i0 = item0 + AT * PER; i0 < rows * (to - t0); i0 += AT * PER) {
-            fetch(t0, to, i0);
-            put(t0, to, i0, xt);
+        put(first, t0, to, xt);
+        for (int i0 = item0 + AT * PER; i0 < full; i0 += AT * PER) {
+            const Items w = items(i0, full);
+            fetch(w, t0);
+            put(w, t0, to, xt);
         }
     };
     if (wk < turns) load(wk);
-    fetch(0, min(turns, cturns), item0);
+    fetch(first, 0);
     fill(0, min(turns, cturns), stage0);
-    if (cturns < turns) fetch(cturns, min(turns, 2 * cturns), item0);
+    if (cturns < turns) fetch(first, cturns);
     __syncthreads();
     int mine = wk; // this wave's next turn
     for (int t0 = 0, at = 0; t0 < turns; t0 += cturns, at ^= 1) {
@@ -408,10 +425,10 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
             }
         }
         if (to < turns) {
-            const int t1 = min(turns, to + cturns), t2 = min(turns, t1 + cturns);
+            const int t1 = min(turns, to + cturns);
             if (!TWO) __syncthreads(); // the one stage is being read
             fill(to, t1, stage0 + (TWO ? (at ^ 1) * stage_bytes : 0));
-            if (t1 < turns) fetch(t1, t2, item0);
+            if (t1 < turns) fetch(first, t1);
             __syncthreads();
         }
     }
