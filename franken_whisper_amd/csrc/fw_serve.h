@@ -39,6 +39,17 @@ static inline bool fw_overlap(const void *a, int64_t na, const void *b, int64_t 
     return na > 0 && nb > 0 && x < y + (uint64_t)nb && y < x + (uint64_t)na;
 }
 
+// Two arrays of `rows` rows of na and nb elements (of `bytes` bytes each): whether
+// they share an element.  Columns of one wider array (equal strides) lie between
+// each other and share none.
+static inline bool fw_rows_overlap(const void *a, int64_t lda, int64_t na, const void *b, int64_t ldb, int64_t nb,
+                                   int64_t rows, int bytes) {
+    if (!fw_overlap(a, ((rows - 1) * lda + na) * bytes, b, ((rows - 1) * ldb + nb) * bytes)) return false;
+    if (rows == 1 || lda != ldb || na > lda || nb > lda) return true;
+    const int64_t row = lda * bytes, d = (((int64_t)((uintptr_t)b - (uintptr_t)a)) % row + row) % row; // b's columns begin d behind a's
+    return d < na * bytes || row - d < nb * bytes;
+}
+
 // The context's device for the length of a call; the caller's comes back.
 struct FwOnDevice {
     int before = -1;

@@ -49,7 +49,7 @@ __device__ __forceinline__ f4 q4_quarters(float v) {
     return f4{__uint_as_float(e[0]), __uint_as_float(o[0]), __uint_as_float(e[1]), __uint_as_float(o[1])};
 }
 
-// Eight codes as operands of a product, in the order q4_unit gives the inputs.
+// Eight codes as operands of a product, in the order of a unit's inputs (below).
 // f16: a code in the low bits of 1024 (or, four bits up, of 64) is that number
 // plus the code; what is too much is taken off again, exactly, and with it the
 // 8 of weights without minimums.
@@ -137,12 +137,22 @@ __device__ __forceinline__ float q4_one(const Q4P &p, int m, int n) {
 }
 
 // The kernel: MT * 16 rows of x by WN waves of NT * 16 outputs each, WK waves
-// taking turns of MS steps of the same outputs.  x is staged in LDS for up to
-// `chunk` inputs at a time, its sums beside it where weights have a minimum (all
-// of x where it fits, else in two stages that take turns); each wave streams its weights straight to registers, one turn ahead.  GB: the
-// 32-weight blocks of a group.  Of a turn's 4 MS blocks a lane quarter loads the
-// scales of its MS, which the quarters then exchange.
-template <typename T, bool MIN, int GB, int MT, int NT, int WN, int WK, int MS, bool TWO>
+// taking turns of MS steps of the same outputs.  Each weight is read once, and
+// straight into the registers that multiply it, a turn ahead; x is what many
+// lanes need, so it goes through LDS: all of it where it fits, else in two stages
+// of `chunk` inputs, one on its way while the other is read.  Beside x lie its
+// sums, where weights have a minimum: what the minimums (and the offsets of the
+// codes) add is one more small product, of sums and scales.  GB: the 32-weight
+// blocks of a group.  Of a turn's 4 MS blocks a lane quarter loads the scales of
+// its MS, which the quarters then exchange.
+//
+// Bound by the weights' bytes up to about 16 rows: one row through 28,672 x 8,192
+// (bf16, groups of 128 with minimums) takes 29 us, 4.3 TB/s where the same access
+// alone takes 24 (4.9), sixteen rows 40 us: staging x for 224 blocks is the rest.
+// With more rows by the instructions around the products (unpacking, scales): 1,500
+// rows through 5,120 x 1,280 (f16, groups of 32 with minimums) take 60 us, 330
+// TFLOP/s; 2,048 through 8,192 x 4,096 (bf16, groups of 128) 264 us, 520 TFLOP/s.
+template <typename T, bool MIN, int GB, int MT, int NT, int WN, int WK, int MS>
 __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
     constexpr bool BF = std::is_same<T, fw_bf16>::value, F32 = std::is_same<T, float>::value, CORR = MIN || BF;
     constexpr int PARTS = Q4X<T>::PARTS, NW = WN * WK, R = MT * 16;
@@ -166,8 +176,10 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
     for (int x = 0; x < MT; x++)
 #pragma unroll
         for (int y = 0; y < NT; y++) acc[x][y] = f4{};
-    if (CORR)
+    if constexpr (CORR) {
         for (int i = threadIdx.x; i < R; i += 64 * NW) odd[i] = 0;
+        __syncthreads(); // before a wave that stages x marks a row
+    }
 
     const int groups = p.k / (32 * GB), blocks = p.k / 32;
     const uint8_t *qrow[NT];
@@ -257,7 +269,7 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
 #pragma unroll
         for (int j = 0; j < AT; j++) {
             const int t = w.t[j], r = w.r[j];
-            if (t < to - t0) {
+            if (t >= to - t0) continue;
             if (!inside(w, t0, j)) {
                 xe[j].clear();
                 xh[j].clear();
@@ -310,7 +322,6 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
                 *(u4 *)to_lds = u4{__builtin_amdgcn_perm(e.y, e.x, 0x05040100), __builtin_amdgcn_perm(h.y, h.x, 0x05040100),
                                    __builtin_amdgcn_perm(e.y, e.x, 0x07060302), __builtin_amdgcn_perm(h.y, h.x, 0x07060302)};
             }
-            }
         }
     };
 
@@ -333,7 +344,7 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
     int mine = wk; // this wave's next turn
     for (int t0 = 0, at = 0; t0 < turns; t0 += cturns, at ^= 1) {
         const int to = min(turns, t0 + cturns);
-        const char *xt = stage0 + (TWO ? at * stage_bytes : 0);
+        const char *xt = stage0 + at * stage_bytes;
         const float *sums = (const float *)(xt + PARTS * plane), *scal = sums + (CORR ? cturns * MS * 4 * R : 0);
 
         const char *xl[MT]; // this lane's units of each row tile (the last row again behind the end)
@@ -426,8 +437,7 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
         }
         if (to < turns) {
             const int t1 = min(turns, to + cturns);
-            if (!TWO) __syncthreads(); // the one stage is being read
-            fill(to, t1, stage0 + (TWO ? (at ^ 1) * stage_bytes : 0));
+            fill(to, t1, stage0 + (at ^ 1) * stage_bytes);
             if (t1 < turns) fetch(first, t1);
             __syncthreads();
         }
@@ -470,21 +480,20 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
     }
 }
 
-template <typename T, bool MIN, int GB, int MT, int NT, int WN, int WK, int MS, bool TWO>
+template <typename T, bool MIN, int GB, int MT, int NT, int WN, int WK, int MS>
 static void q4_go(hipStream_t st, Q4P p) {
     constexpr bool CORR = MIN || std::is_same<T, fw_bf16>::value, F32 = std::is_same<T, float>::value;
     const int rows = std::min(p.m, MT * 16);
-    // All of x in one stage where it fits 64 KiB of LDS; else TWO stages, of whole
+    // All of x in one stage where it fits 64 KiB of LDS; else two stages, of whole
     // rounds of the waves' turns in 80 KiB together (two blocks a CU) where one
-    // fits, of as many turns as 144 KiB hold where not; or one of 64 KiB that is
-    // filled again.
+    // fits, of as many turns as 144 KiB hold where not.
     const int turn = MS * (Q4X<T>::PARTS * rows * 256 + (CORR ? 256 * MT : 0)) + (F32 ? 64 * MT : 0);
     const int fixed = Q4X<T>::PARTS * rows * 16, join = WK > 1 ? WN * WK * MT * NT * 1024 : 0;
     const int all_turns = (p.k + 128 * MS - 1) / (128 * MS);
     int turns = all_turns, stages = 1;
     if (turns * (int64_t)turn + fixed > 65536) {
-        stages = TWO ? 2 : 1;
-        turns = ((TWO ? 40960 : 65536) - fixed) / turn / WK * WK;
+        stages = 2;
+        turns = (40960 - fixed) / turn / WK * WK;
         if (turns < 1) turns = std::max(1, std::min(WK, (73728 - fixed) / turn));
     }
     p.chunk = turns * MS * 128;
@@ -496,36 +505,36 @@ static void q4_go(hipStream_t st, Q4P p) {
         p.x = (const T *)all.x + at * all.ldx;
         p.y = (T *)all.y + at * all.ldy;
         const dim3 grid((unsigned)((p.n + 16 * NT * WN - 1) / (16 * NT * WN)), (unsigned)((p.m + 16 * MT - 1) / (16 * MT)));
-        hipLaunchKernelGGL((k_q4<T, MIN, GB, MT, NT, WN, WK, MS, TWO>), grid, dim3(64 * WN * WK), p.lds, st, p);
+        hipLaunchKernelGGL((k_q4<T, MIN, GB, MT, NT, WN, WK, MS>), grid, dim3(64 * WN * WK), p.lds, st, p);
     }
 }
 // Which form runs.  x is staged once a block, so many outputs a block save
 // staging; few outputs a block spread a small weight over the chip, its waves
 // then sharing outputs and taking turns of the inputs.  Longer turns (512
 // inputs, not 128) carry fewer scale loads and waits but leave more idle at the
-// end of short rows.  Measured both sides of each border, us, this form / the next:
+// end of short rows.  Measured on both sides, us, the form that runs / the other:
 //   1..16 rows, up to 640 tiles of 16 outputs: 1 x 5120 x 1280 5.2 / 7.9
-//     k < 2048: 10 x 51866 x 1280 (f32) 18.5 / 32;  1 x 51866 x 1280 13.1 / 20
-//     up to 1280 tiles: 8 x 14336 x 4096 14.3 / 18.8;  above: 16 x 28672 x 8192 49 / 44
-//   17..32 rows: 20 x 1280 x 1280 7.3 / 8.0;  32 x 5120 x 1280 (f32) 15.9 / 21;  32 x 28672 x 8192 99 / 63
-//   more, in tiles of 64 rows, by how many blocks there are: 1500 x 5120 x 1280 58 / 70;
-//     256 x 5120 x 5120 106 / 90;  64 x 5120 x 5120 70 / 50
+//     k < 2048: 10 x 51866 x 1280 (f32) 18.5 / 32, 1 x 51866 x 1280 13 / 20
+//     up to 1280 tiles: 8 x 14336 x 4096 14.3 / 18.8; above: 16 x 28672 x 8192 44 / 49
+//   17..32 rows: 20 x 1280 x 1280 7.3 / 8.0, 32 x 5120 x 1280 (f32) 15.9 / 21, 32 x 28672 x 8192 63 / 99
+//   more, in tiles of 64 rows, by how many blocks there are: 1500 x 5120 x 1280 58 / 70,
+//     256 x 5120 x 5120 90 / 106, 64 x 5120 x 5120 50 / 70
 template <typename T, bool MIN, int GB>
 static void q4_rows(hipStream_t st, const Q4P &p) {
     const int64_t tiles = (p.n + 15) / 16, mt = (p.m + 63) / 64;
     if (p.m <= 16) {
-        if (tiles <= 640) q4_go<T, MIN, GB, 1, 1, 1, 8, 1, true>(st, p);
-        else if (p.k < 2048) q4_go<T, MIN, GB, 1, 1, 8, 1, 2, true>(st, p);
-        else if (tiles <= 1280) q4_go<T, MIN, GB, 1, 1, 4, 2, 4, true>(st, p);
-        else q4_go<T, MIN, GB, 1, 1, 8, 1, 4, true>(st, p);
+        if (tiles <= 640) q4_go<T, MIN, GB, 1, 1, 1, 8, 1>(st, p);
+        else if (p.k < 2048) q4_go<T, MIN, GB, 1, 1, 8, 1, 2>(st, p);
+        else if (tiles <= 1280) q4_go<T, MIN, GB, 1, 1, 4, 2, 4>(st, p);
+        else q4_go<T, MIN, GB, 1, 1, 8, 1, 4>(st, p);
     } else if (p.m <= 32) {
-        if (tiles <= 128) q4_go<T, MIN, GB, 2, 1, 1, 8, 1, true>(st, p);
-        else if (tiles <= 512) q4_go<T, MIN, GB, 2, 1, 2, 4, 1, true>(st, p);
-        else q4_go<T, MIN, GB, 2, 1, 8, 1, 2, true>(st, p);
-    } else if ((tiles + 15) / 16 * mt >= 256) q4_go<T, MIN, GB, 4, 2, 8, 1, 1, true>(st, p);
-    else if ((tiles + 7) / 8 * mt >= 128) q4_go<T, MIN, GB, 4, 1, 8, 1, 2, true>(st, p);
-    else if ((tiles + 3) / 4 * mt >= 96) q4_go<T, MIN, GB, 4, 1, 4, 2, 2, true>(st, p);
-    else q4_go<T, MIN, GB, 4, 1, 2, 4, 1, true>(st, p);
+        if (tiles <= 128) q4_go<T, MIN, GB, 2, 1, 1, 8, 1>(st, p);
+        else if (tiles <= 512) q4_go<T, MIN, GB, 2, 1, 2, 4, 1>(st, p);
+        else q4_go<T, MIN, GB, 2, 1, 8, 1, 2>(st, p);
+    } else if ((tiles + 15) / 16 * mt >= 256) q4_go<T, MIN, GB, 4, 2, 8, 1, 1>(st, p);
+    else if ((tiles + 7) / 8 * mt >= 128) q4_go<T, MIN, GB, 4, 1, 8, 1, 2>(st, p);
+    else if ((tiles + 3) / 4 * mt >= 96) q4_go<T, MIN, GB, 4, 1, 4, 2, 2>(st, p);
+    else q4_go<T, MIN, GB, 4, 1, 2, 4, 1>(st, p);
 }
 template <typename T>
 static void q4_type(hipStream_t st, const Q4P &p) {
@@ -549,6 +558,8 @@ extern "C" fwhip_status fwhip_q4_linear(fwhip_ctx *c, const fwhip_q4_linear_args
         return fw_fail(FWHIP_ERR_UNSUPPORTED, "fwhip_q4_linear: group must be 32, 64 or 128");
     if (a->m < 0 || a->n < 0 || a->k < a->group || a->k % a->group)
         return fw_fail(FWHIP_ERR_INVALID, "fwhip_q4_linear: m, n >= 0 and k a positive multiple of group");
+    if (a->k > 1 << 24 || a->n > 1 << 29)
+        return fw_fail(FWHIP_ERR_UNSUPPORTED, "fwhip_q4_linear: k above 2^24 or n above 2^29");
     if (a->ldx < a->k || a->ldy < a->n) return fw_fail(FWHIP_ERR_INVALID, "fwhip_q4_linear: ldx < k or ldy < n");
     if (a->m && a->n) {
         if (!a->x || !a->q || !a->scale || !a->y) return fw_fail(FWHIP_ERR_INVALID, "fwhip_q4_linear: NULL argument");
@@ -557,8 +568,7 @@ extern "C" fwhip_status fwhip_q4_linear(fwhip_ctx *c, const fwhip_q4_linear_args
         if (!fw_aligned(a->x, eb) || !fw_aligned(a->y, eb) || !fw_aligned(a->scale, sb) || !fw_aligned(a->minimum, sb) ||
             !fw_aligned(a->bias, 4))
             return fw_fail(FWHIP_ERR_INVALID, "fwhip_q4_linear: an address is not a multiple of its element's size");
-        if (fw_overlap(a->y, ((a->m - 1) * a->ldy + a->n) * eb, a->x, ((a->m - 1) * a->ldx + a->k) * eb) &&
-            (a->ldx != a->ldy || a->x == a->y))
+        if (fw_rows_overlap(a->y, a->ldy, a->n, a->x, a->ldx, a->k, a->m, eb))
             return fw_fail(FWHIP_ERR_INVALID, "fwhip_q4_linear: y must not overlap x");
     }
     if (!c) return fw_fail(FWHIP_ERR_INVALID, "fwhip_q4_linear: NULL ctx");

@@ -914,7 +914,9 @@ extern "C" fwhip_status fwhip_tree_attn(fwhip_ctx *c, const fwhip_tree_attn_args
         for (int k = 1; k < 8; k++)
             if (strides[k] * eb % 16)
                 return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn: strides must be multiples of 16 bytes");
-        if (a->out == a->q) return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn: out must not be q");
+        const int64_t qn = (a->n_heads - 1) * a->q_head + a->head_dim, on = (a->n_heads - 1) * a->out_head + a->head_dim;
+        if (fw_rows_overlap(a->out, a->out_row, on, a->q, a->q_row, qn, a->n_rows, eb))
+            return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn: out must not overlap q");
     }
     if (a->page_stride > 0x3fffffff || a->token_stride > 0x3fffffff)
         return fw_fail(FWHIP_ERR_UNSUPPORTED, "fwhip_tree_attn: page and token strides must be below 2^30 elements");

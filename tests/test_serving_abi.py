@@ -90,7 +90,7 @@ def test_append_refusals(kw, word):
     (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(q_row=-8), "negative stride"), (dict(table_stride=-1), "negative stride"), (dict(q=None), "NULL"),
     (dict(table=None), "NULL"), (dict(row_start=None), "NULL"), (dict(len=None), "NULL"), (dict(out=None), "NULL"),
     (dict(k_cache=None), "NULL"), (dict(q=A + 8), "16-byte"), (dict(v_cache=3 * A + 4), "16-byte"),
-    (dict(q_head=4), "multiples of 16"), (dict(page_stride=2047), "multiples of 16"), (dict(out=A), "out must not"),
+    (dict(q_head=4), "multiples of 16"), (dict(page_stride=2047), "multiples of 16"), (dict(out=A), "out must not"), (dict(out=A + 16), "out must not"),
     (dict(mask_words=0), "mask"), (dict(max_new=65), "mask"), (dict(mask=None), "mask"),
 ])
 def test_attention_refusals(kw, word):
@@ -139,7 +139,11 @@ def test_attention_workspace_is_checked():
     (dict(x=None), "NULL", abi.ERR_INVALID), (dict(q=None), "NULL", abi.ERR_INVALID), (dict(y=None), "NULL", abi.ERR_INVALID),
     (dict(scale=None), "NULL", abi.ERR_INVALID), (dict(q=2 * A + 8), "16-byte", abi.ERR_INVALID),
     (dict(x=A + 1), "address", abi.ERR_INVALID), (dict(bias=4 * A + 2), "address", abi.ERR_INVALID),
-    (dict(y=A), "overlap", abi.ERR_INVALID),
+    (dict(y=A), "overlap", abi.ERR_INVALID), (dict(y=A + 2), "overlap", abi.ERR_INVALID),
+    (dict(y=A + 128 - 2, ldx=200, ldy=200), "overlap", abi.ERR_INVALID), (dict(y=A - 98, ldx=200, ldy=200), "overlap", abi.ERR_INVALID),
+    (dict(y=A + 200, ldx=200, ldy=210), "overlap", abi.ERR_INVALID), (dict(y=A + 128, ldx=114, ldy=114), "NULL ctx", abi.ERR_INVALID),
+    (dict(y=A + 126, ldx=114, ldy=114), "overlap", abi.ERR_INVALID), (dict(y=A - 100, ldx=114, ldy=114), "NULL ctx", abi.ERR_INVALID),
+    (dict(k=(1 << 24) + 32, ldx=1 << 25), "2^24", abi.ERR_UNSUPPORTED), (dict(n=(1 << 29) + 1, ldy=1 << 30), "2^29", abi.ERR_UNSUPPORTED),
 ])
 def test_linear_refusals(kw, word, code):
     _says("fwhip_q4_linear", _set(_q4, **kw), word, code)
