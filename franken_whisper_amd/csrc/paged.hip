@@ -174,6 +174,13 @@ extern "C" fwhip_status fwhip_paged_plan(fwhip_ctx *c, const fwhip_paged_plan_ar
     if (a->mask_words < 0 || a->mask_words > FWP_MASK_WORDS ||
         (tree ? a->n_rows && (!a->parents || !a->mask) : a->parents || a->mask))
         return fw_fail(FWHIP_ERR_INVALID, "fwhip_paged_plan: parents and mask go together, with mask_words in 1..4");
+    for (const void *v : {(const void *)a->len, (const void *)a->n_new, (const void *)a->parents, (const void *)a->table,
+                          (const void *)a->held, (const void *)a->free_pages, (const void *)a->free_count,
+                          (const void *)a->table_out, (const void *)a->held_out, (const void *)a->count_out,
+                          (const void *)a->row_start, (const void *)a->row_req, (const void *)a->pos, (const void *)a->status})
+        if (!fw_aligned(v, 4)) return fw_fail(FWHIP_ERR_INVALID, "fwhip_paged_plan: an address is not a multiple of its element's size");
+    if (!fw_aligned(a->slot, 8) || !fw_aligned(a->mask, 8))
+        return fw_fail(FWHIP_ERR_INVALID, "fwhip_paged_plan: an address is not a multiple of its element's size");
     // every block reads the lengths that other blocks' results would replace
     if (a->n_req && (fw_overlap(a->held_out, 4ll * a->n_req, a->held, 4ll * a->n_req) ||
                      fw_overlap(a->held_out, 4ll * a->n_req, a->len, 4ll * a->n_req) ||

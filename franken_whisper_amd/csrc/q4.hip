@@ -83,7 +83,8 @@ __device__ __forceinline__ u4 q4_codes_bf16(uint32_t w, Q4Magic k) {
 // of 8, the unit (block, c) holding inputs 4 c + 0, 2, 16, 18, 1, 3, 17, 19 of its
 // block.  f16 and bf16 as they are; f32 as two f16 parts of x / s, where s is
 // the power of two that takes the largest |x| of the row's turn of inputs to
-// 2^14..2^15: hi + lo is within 2^-22 of x down to 2^-28 of that largest.
+// 2^14..2^15: hi + lo is within 2^-22 of x, or 2^-39 of that largest (where the
+// second part falls below f16's normal numbers).
 template <typename T>
 struct Q4X {
     static constexpr int PARTS = std::is_same<T, float>::value ? 2 : 1;
@@ -166,8 +167,7 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
     const int cturns = p.chunk / (128 * MS), turns = (p.k + 128 * MS - 1) / (128 * MS);
     const int xrow = p.chunk * 2 + 16; // bytes of a row: rows 4 banks apart
     const int plane = rows * xrow;
-    int *odd = (int *)lds;    // [R]: rows with a value that is not finite
-    char *stage0 = lds + R * 4; // one or two stages: x [part][row][xrow], CORR: sums [turn][MS][4][R], f32: scales [turn][R]
+    char *stage0 = lds; // one or two stages: x [part][row][xrow], CORR: sums [turn][MS][4][R], f32: scales [turn][R]
     Q4Magic magic = BF ? Q4Magic{0x43004300u, 0} : Q4Magic{0x64006400u, 0x54005400u};
     asm volatile("" : "+v"(magic.lo), "+v"(magic.hi));
 
@@ -176,10 +176,6 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
     for (int x = 0; x < MT; x++)
 #pragma unroll
         for (int y = 0; y < NT; y++) acc[x][y] = f4{};
-    if constexpr (CORR) {
-        for (int i = threadIdx.x; i < R; i += 64 * NW) odd[i] = 0;
-        __syncthreads(); // before a wave that stages x marks a row
-    }
 
     const int groups = p.k / (32 * GB), blocks = p.k / 32;
     const uint8_t *qrow[NT];
@@ -279,7 +275,6 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
                 float v = xh[j].sum(xe[j].sum(0.0f));
                 v = v + fw_dpp_f32<FW_DPP_XOR1>(v);
                 v = v + fw_dpp_f32<FW_DPP_XOR2>(v);
-                if (!(fabsf(v) < INFINITY)) odd[r] = 1;
                 if constexpr (GB >= 2 && MS >= 2) v = v + fw_dpp_f32<FW_DPP_HALF_MIRROR>(v);
                 if constexpr (GB >= 4 && MS >= 4) v = v + fw_dpp_f32<FW_DPP_MIRROR>(v);
                 // block b of the turn: quarter b / MS, its scale (b % MS) / GB
@@ -473,8 +468,8 @@ __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
                 const int r = x * 16 + 4 * c + j;
                 if (r >= rows) continue;
                 float v = acc[x][y][j];
-                // sums of inputs that are not finite do not come apart again: product by product
-                if (CORR && odd[r]) v = q4_one<T, MIN>(p, m0 + r, n);
+                // what an infinity or NaN, or a sum that overflowed on its way, left: once more, product by product
+                if (__builtin_expect(!(fabsf(v) < INFINITY), 0)) v = q4_one<T, MIN>(p, m0 + r, n);
                 ((T *)p.y)[(int64_t)(m0 + r) * p.ldy + n] = fw_cvt<T>(v + bias);
             }
     }
@@ -498,7 +493,7 @@ static void q4_go(hipStream_t st, Q4P p) {
     }
     p.chunk = turns * MS * 128;
     p.stage = turns * turn + fixed;
-    p.lds = 64 * MT + std::max(stages * p.stage, join);
+    p.lds = std::max(stages * p.stage, join);
     const Q4P all = p;
     for (int64_t at = 0; at < all.m; at += 65535 * 16 * MT) { // the grid's reach in rows
         p.m = (int)std::min<int64_t>(all.m - at, 65535 * 16 * MT);

@@ -493,7 +493,7 @@ __device__ __forceinline__ void tree_slow(const TreeP &p, const TreeBlock &b, ch
         const int i = t / b.group, h = b.kvh * b.group + t % b.group;
         const T *q = (const T *)p.q + (int64_t)(b.rq.row0 + i) * p.q_row + h * p.q_head;
         wave_fence();
-        for (int e = lane; e < D; e += 64) sq[e] = fw_to_f32(q[e]);
+        for (int e = lane; e < D; e += 64) sq[e] = fw_to_f32(q[e]) * (p.scale == 0.0f ? 0.0f : 1.0f); // as tree_query
         wave_fence();
         float m = -INFINITY, l = 0.0f, o[D / 64] = {};
         for (int j0 = b.first; j0 < b.last; j0 += 64) {
@@ -914,6 +914,8 @@ extern "C" fwhip_status fwhip_tree_attn(fwhip_ctx *c, const fwhip_tree_attn_args
         for (int k = 1; k < 8; k++)
             if (strides[k] * eb % 16)
                 return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn: strides must be multiples of 16 bytes");
+        if (!fw_aligned(a->table, 4) || !fw_aligned(a->len, 4) || !fw_aligned(a->row_start, 4) || !fw_aligned(a->mask, 8))
+            return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn: an address is not a multiple of its element's size");
         const int64_t qn = (a->n_heads - 1) * a->q_head + a->head_dim, on = (a->n_heads - 1) * a->out_head + a->head_dim;
         if (fw_rows_overlap(a->out, a->out_row, on, a->q, a->q_row, qn, a->n_rows, eb))
             return fw_fail(FWHIP_ERR_INVALID, "fwhip_tree_attn: out must not overlap q");

@@ -685,7 +685,8 @@ fwhip_status fwhip_decoder_load_ggml(fwhip_ctx *ctx, const fwhip_ggml *g, int32_
  *
  * All four only queue work on the context's stream: they allocate nothing,
  * wait for nothing and copy nothing to the host, so a step can be captured
- * into a HIP graph.  Pointers are device addresses.  What the host can see is
+ * into a HIP graph (on a context that was made before the capture began).
+ * Pointers are device addresses, multiples of their elements' size.  What the host can see is
  * checked before anything is queued (FWHIP_ERR_INVALID, or
  * FWHIP_ERR_UNSUPPORTED for a form that is not built); what only the device
  * knows (lengths, page numbers, slots) is checked by the kernels, which never
@@ -704,9 +705,10 @@ fwhip_status fwhip_decoder_load_ggml(fwhip_ctx *ctx, const fwhip_ggml *g, int32_
  *   pages     request r needs ceil((len + n_new) / page_size) - held more pages
  *             when that is positive.  Requests take them in order from the top
  *             of the free list (free_pages[count - 1] first) for as long as the
- *             running sum of needs stays within count; one that does not fit,
- *             or whose table row has no room, gets none (status 1), and so do
- *             all later ones that need pages.
+ *             running sum of needs stays within count; one that does not fit
+ *             gets none (status 1), and so do all later ones that need pages.
+ *             One whose table row has no room gets none either (status 1) and
+ *             leaves the pages to the others.
  *   rows      the new tokens of all requests in order: row_start [n_req + 1],
  *             and per row row_req (its request), slot (page * page_size +
  *             offset, -1 when its request got no pages) and pos.
@@ -768,15 +770,21 @@ fwhip_status fwhip_paged_append(fwhip_ctx *ctx, const fwhip_paged_append_args *a
  * outside [row_start[0], row_start[n_req]) are neither read nor written.
  * Query head h reads K/V head h / (n_heads / n_kv_heads).
  * max_new and max_len bound a request's new tokens and its len + new tokens
- * (the host's view of the step: larger ones only cost time).  Rows of a request
+ * (the host's view of the step: larger ones only cost time; max_len <= width *
+ * page_size, and the sums over a long cache are cut by them, so results may
+ * differ in the last bits between two bounds).  Rows of a request
  * that exceeds a bound, has a negative length, or sees a token whose table entry
  * is no page of [0, n_pages) come out as NaN; such entries are never followed.
  * q, the caches and out share one type; scores, softmax and sums are f32.
- * head_dim is 64 or 128; addresses and strides are multiples of 16 bytes, the
- * strides non-negative.  workspace (16-byte aligned) holds the partial results
+ * scale is finite; of either sign, or zero.
+ * head_dim is 64 or 128; addresses and strides of q, the caches and out are
+ * multiples of 16 bytes, the strides non-negative, page_stride and token_stride
+ * below 2^30 elements; n_req < 65536, n_pages >= 1, and n_kv_heads x ceil(max_new
+ * x group / 128) <= 2^23.  workspace (16-byte aligned) holds the partial results
  * of a long cache that is split over workgroups: at least
- * fwhip_tree_attn_workspace bytes for the same sizes, and for the call alone
- * until it has run (two graphs that may replay at once need one each). */
+ * fwhip_tree_attn_workspace bytes for the same sizes (0 up to max_len 512), and
+ * for the call alone until it has run (two graphs that may replay at once need
+ * one each). */
 typedef struct fwhip_tree_attn_args {
     int32_t dtype;                     /* FWHIP_T_* */
     int32_t n_req, n_rows;             /* requests; rows of q and out */
@@ -807,8 +815,13 @@ fwhip_status fwhip_tree_attn_workspace(int32_t n_req, int32_t n_heads, int32_t n
  * optionally a minimum, for every `group` weights of a row ([n, k / group]):
  *   w = (code - 8) * scale, or code * scale + minimum.
  * x and y share a type.  Codes are multiplied as whole numbers, summed per group
- * in f32 and scaled in f32; y is rounded once.
- * group is 32, 64 or 128 and divides k; q 16-byte aligned, ldx >= k, ldy >= n. */
+ * in f32 and scaled in f32; y is rounded once.  f32 inputs are multiplied as two
+ * 16-bit parts: exact to 2^-22, or to 2^-39 of the largest of the 128 to 512
+ * inputs of the row around them.  An input that is not finite stays in its row,
+ * and its outputs are those of the sum of products.
+ * group is 32, 64 or 128 and divides k; k <= 2^24, n <= 2^29; q 16-byte aligned,
+ * ldx >= k, ldy >= n.  y shares no element with x, but may be columns between
+ * x's columns of one wider array (ldx = ldy). */
 typedef struct fwhip_q4_linear_args {
     int32_t dtype, scale_dtype;        /* of x and y: FWHIP_T_*; of the planes: FWHIP_T_F16 or FWHIP_T_F32 */
     int32_t group, m, n, k;

@@ -538,6 +538,40 @@ def test_q4_linear_values_far_apart(tctx, kind):
         assert (np.sign(got[exact_inf]) == sign * np.sign(w[exact_inf, e])).all()
 
 
+@pytest.mark.parametrize("kind", DT)
+@pytest.mark.parametrize("m,n,k,group,minimum", [(3, 40, 512, 128, True), (20, 40, 1024, 128, False), (70, 100, 256, 32, True)])
+def test_q4_linear_near_the_ends_of_the_type(tctx, kind, m, n, k, group, minimum):
+    """Sums that overflow on their way to a finite result, and inputs below the
+    type's normal numbers (every sum counts what each of them is worth)."""
+    x, q, s, mn, b = q4_inputs(m, kind, m, n, k, group, minimum, False, "f32")
+    if kind == "f16":
+        x = (x.clamp(-4, 4) * 2.0 ** -18).to(torch.float16)  # steps of 2^-24: few bits each, all exact in the oracle too
+        s, mn = s * 2.0 ** 12, None if mn is None else mn * 2.0 ** 12
+    else:
+        x = (x.float() * 2.0 ** 124).clamp(-2.0 ** 126, 2.0 ** 126).to(DT[kind])
+        s, mn = s * 2.0 ** -20, None if mn is None else mn * 2.0 ** -20
+    check_q4(tctx, kind, x, q, s, mn, b, group)
+
+
+def test_attention_scale_zero_beside_infinities(tctx):
+    """A scale of zero weighs all seen keys alike; rows in one tile with a row
+    that is not finite give what they give alone."""
+    s = attn_inputs(31, "f32", [40], [4], 4, 1, 64, 16, False)
+    s["scale"] = 0.0
+    rs = s["row_start"]
+    s["q"][int(rs[0])] = 3e38
+    want, tol = reference(s)
+    s["q"][int(rs[0]) + 2, 1, 5] = float("inf")
+    got = run_attn(tctx, s)
+    for i in range(4):
+        for h in range(4):
+            if (i, h) == (2, 1):
+                assert torch.isnan(got[int(rs[0]) + i, h]).all()
+            else:
+                d = np.abs(host(got[int(rs[0]) + i, h]) - want[int(rs[0]) + i, h])
+                assert (d <= tol[int(rs[0]) + i, h]).all(), (i, h, d.max())
+
+
 def test_q4_linear_of_nothing(tctx):
     _, q, s, _, _ = q4_inputs(4, "f32", 1, 8, 64, 32, False, False)
     ops.q4_linear(tctx, torch.empty(0, 64).cuda(), q.cuda(), s.cuda(), torch.empty(0, 8).cuda())

@@ -58,6 +58,8 @@ def test_a_good_call_gets_as_far_as_its_context(fn, make):
     (dict(mask_words=0), "mask_words"), (dict(mask_words=5), "mask_words"),
     (dict(held_out=A + 0x40000), "held_out"), (dict(held_out=A), "held_out"), (dict(count_out=A + 0x60000), "count_out"),
     (dict(table_out=A + 0x30000 + 4), "table_out"),
+    (dict(status=A + 2), "address"), (dict(parents=A + 1), "address"), (dict(free_count=A + 3), "address"),
+    (dict(slot=A + 4), "address"), (dict(mask=A + 4), "address"),
 ])
 def test_plan_refusals(kw, word):
     _says("fwhip_paged_plan", _set(_plan, **kw), word)
@@ -92,6 +94,7 @@ def test_append_refusals(kw, word):
     (dict(k_cache=None), "NULL"), (dict(q=A + 8), "16-byte"), (dict(v_cache=3 * A + 4), "16-byte"),
     (dict(q_head=4), "multiples of 16"), (dict(page_stride=2047), "multiples of 16"), (dict(out=A), "out must not"), (dict(out=A + 16), "out must not"),
     (dict(mask_words=0), "mask"), (dict(max_new=65), "mask"), (dict(mask=None), "mask"),
+    (dict(table=A + 2), "address"), (dict(len=A + 1), "address"), (dict(row_start=A + 2), "address"), (dict(mask=A + 4), "address"),
 ])
 def test_attention_refusals(kw, word):
     _says("fwhip_tree_attn", _set(_attn, **kw), word)
