@@ -151,8 +151,8 @@ __device__ __forceinline__ float q4_one(const Q4P &p, int m, int n) {
 // (bf16, groups of 128 with minimums) takes 29 us, 4.3 TB/s where the same access
 // alone takes 24 (4.9), sixteen rows 40 us: staging x for 224 blocks is the rest.
 // With more rows by the instructions around the products (unpacking, scales): 1,500
-// rows through 5,120 x 1,280 (f16, groups of 32 with minimums) take 60 us, 330
-// TFLOP/s; 2,048 through 8,192 x 4,096 (bf16, groups of 128) 264 us, 520 TFLOP/s.
+// rows through 5,120 x 1,280 (f16, groups of 32 with minimums) take 58 us, 336
+// TFLOP/s; 2,048 through 8,192 x 4,096 (bf16, groups of 128) 255 us, 538 TFLOP/s.
 template <typename T, bool MIN, int GB, int MT, int NT, int WN, int WK, int MS>
 __global__ void __launch_bounds__(64 * WN * WK) k_q4(Q4P p) {
     constexpr bool BF = std::is_same<T, fw_bf16>::value, F32 = std::is_same<T, float>::value, CORR = MIN || BF;
@@ -503,33 +503,36 @@ static void q4_go(hipStream_t st, Q4P p) {
         hipLaunchKernelGGL((k_q4<T, MIN, GB, MT, NT, WN, WK, MS>), grid, dim3(64 * WN * WK), p.lds, st, p);
     }
 }
-// Which form runs.  x is staged once a block, so many outputs a block save
-// staging; few outputs a block spread a small weight over the chip, its waves
-// then sharing outputs and taking turns of the inputs.  Longer turns (512
-// inputs, not 128) carry fewer scale loads and waits but leave more idle at the
-// end of short rows.  Measured on both sides, us, the form that runs / the other:
+
+// Which form runs.  x is staged once a block, so many outputs and rows a block
+// save staging and unpacking; few spread a small product over the chip, the waves
+// of a block then sharing outputs and taking turns of the inputs.  Longer turns
+// carry fewer scale loads and waits but leave more idle at the end of short rows.
+// Measured on both sides, us, the form that runs / the next best of the others:
 //   1..16 rows, up to 640 tiles of 16 outputs: 1 x 5120 x 1280 5.2 / 7.9
 //     k < 2048: 10 x 51866 x 1280 (f32) 18.5 / 32, 1 x 51866 x 1280 13 / 20
 //     up to 1280 tiles: 8 x 14336 x 4096 14.3 / 18.8; above: 16 x 28672 x 8192 44 / 49
-//   17..32 rows: 20 x 1280 x 1280 7.3 / 8.0, 32 x 5120 x 1280 (f32) 15.9 / 21, 32 x 28672 x 8192 63 / 99
-//   more, in tiles of 64 rows, by how many blocks there are: 1500 x 5120 x 1280 58 / 70,
-//     256 x 5120 x 5120 90 / 106, 64 x 5120 x 5120 50 / 70
+//   more, by how many blocks of 64 rows x 256 outputs, 32 x 128, 32 x 64 or 32 x 32
+//     there are: 1500 x 5120 x 1280 58 / 71 and 700 x 5120 x 1280 28 / 31;
+//     128 x 8192 x 8192 (groups of 128) 49 / 54, 440 x 3840 x 1280 21 / 23, 128 x 5120 x 1280 13 / 15;
+//     64 x 5120 x 5120 25.7 / 26.0, 100 x 3840 x 1280 (f32) 15 / 18, 300 x 1280 x 1280 9.9 / 10.9;
+//     32 x 8192 x 4096 19 / 24, 24 x 5120 x 5120 19 / 26; then 32 x 16: 20 x 1280 x 1280 6.8 / 7.5
+//   groups of 32: turns of 128 inputs, 256 x 5120 x 5120 57 / 60 with 256; longer groups
+//     (fewer scales in registers): 256, 64 x 14336 x 4096 28 / 34 with 128.
 template <typename T, bool MIN, int GB>
 static void q4_rows(hipStream_t st, const Q4P &p) {
-    const int64_t tiles = (p.n + 15) / 16, mt = (p.m + 63) / 64;
+    constexpr int MS = GB == 1 ? 1 : 2;
+    const int64_t tiles = (p.n + 15) / 16, mt = (p.m + 31) / 32;
     if (p.m <= 16) {
         if (tiles <= 640) q4_go<T, MIN, GB, 1, 1, 1, 8, 1>(st, p);
         else if (p.k < 2048) q4_go<T, MIN, GB, 1, 1, 8, 1, 2>(st, p);
         else if (tiles <= 1280) q4_go<T, MIN, GB, 1, 1, 4, 2, 4>(st, p);
         else q4_go<T, MIN, GB, 1, 1, 8, 1, 4>(st, p);
-    } else if (p.m <= 32) {
-        if (tiles <= 128) q4_go<T, MIN, GB, 2, 1, 1, 8, 1>(st, p);
-        else if (tiles <= 512) q4_go<T, MIN, GB, 2, 1, 2, 4, 1>(st, p);
-        else q4_go<T, MIN, GB, 2, 1, 8, 1, 2>(st, p);
-    } else if ((tiles + 15) / 16 * mt >= 256) q4_go<T, MIN, GB, 4, 2, 8, 1, 1>(st, p);
-    else if ((tiles + 7) / 8 * mt >= 128) q4_go<T, MIN, GB, 4, 1, 8, 1, 2>(st, p);
-    else if ((tiles + 3) / 4 * mt >= 96) q4_go<T, MIN, GB, 4, 1, 4, 2, 2>(st, p);
-    else q4_go<T, MIN, GB, 4, 1, 2, 4, 1>(st, p);
+    } else if ((tiles + 15) / 16 * ((p.m + 63) / 64) >= 216) q4_go<T, MIN, GB, 4, 2, 8, 1, 1>(st, p);
+    else if ((tiles + 7) / 8 * mt >= 150) q4_go<T, MIN, GB, 2, 1, 8, 1, MS>(st, p);
+    else if ((tiles + 3) / 4 * mt >= 140) q4_go<T, MIN, GB, 2, 1, 4, 2, MS>(st, p);
+    else if ((tiles + 1) / 2 * mt >= 64) q4_go<T, MIN, GB, 2, 1, 2, 4, 1>(st, p);
+    else q4_go<T, MIN, GB, 2, 1, 1, 8, 1>(st, p);
 }
 template <typename T>
 static void q4_type(hipStream_t st, const Q4P &p) {
