@@ -512,27 +512,29 @@ static void q4_go(hipStream_t st, Q4P p) {
 //   1..16 rows, up to 640 tiles of 16 outputs: 1 x 5120 x 1280 5.2 / 7.9
 //     k < 2048: 10 x 51866 x 1280 (f32) 18.5 / 32, 1 x 51866 x 1280 13 / 20
 //     up to 1280 tiles: 8 x 14336 x 4096 14.3 / 18.8; above: 16 x 28672 x 8192 44 / 49
-//   more, by how many blocks of 64 rows x 256 outputs, 32 x 128, 32 x 64 or 32 x 32
-//     there are: 1500 x 5120 x 1280 58 / 71 and 700 x 5120 x 1280 28 / 31;
-//     128 x 8192 x 8192 (groups of 128) 49 / 54, 440 x 3840 x 1280 21 / 23, 128 x 5120 x 1280 13 / 15;
-//     64 x 5120 x 5120 25.7 / 26.0, 100 x 3840 x 1280 (f32) 15 / 18, 300 x 1280 x 1280 9.9 / 10.9;
-//     32 x 8192 x 4096 19 / 24, 24 x 5120 x 5120 19 / 26; then 32 x 16: 20 x 1280 x 1280 6.8 / 7.5
+//   more, by how many blocks of 64 rows x 256 outputs, 32 x 128 or 32 x 64 there are,
+//     else of 16 x 64, 16 x 32 or 16 x 16:
+//     1500 x 5120 x 1280 58 / 71 and 700 x 5120 x 1280 28 / 31;
+//     128 x 8192 x 8192 (groups of 128) 49 / 54, 440 x 1280 x 5120 (f32) 62 / 75, 128 x 5120 x 1280 13 / 15;
+//     64 x 5120 x 5120 25.8 / 27.3 (but 200 x 1280 x 5120 in f32, whose staging is twice the work, 47 / 40);
+//     24 x 5120 x 5120 17 / 19, 32 x 5120 x 1280 (f32) 10 / 13; 90 x 1280 x 1280 (f32) 9.2 / 9.9;
+//     24 x 1280 x 5120 (f32) 21 / 23, 20 x 1280 x 1280 5.9 / 6.4
 //   groups of 32: turns of 128 inputs, 256 x 5120 x 5120 57 / 60 with 256; longer groups
 //     (fewer scales in registers): 256, 64 x 14336 x 4096 28 / 34 with 128.
 template <typename T, bool MIN, int GB>
 static void q4_rows(hipStream_t st, const Q4P &p) {
     constexpr int MS = GB == 1 ? 1 : 2;
-    const int64_t tiles = (p.n + 15) / 16, mt = (p.m + 31) / 32;
-    if (p.m <= 16) {
-        if (tiles <= 640) q4_go<T, MIN, GB, 1, 1, 1, 8, 1>(st, p);
-        else if (p.k < 2048) q4_go<T, MIN, GB, 1, 1, 8, 1, 2>(st, p);
+    const int64_t tiles = (p.n + 15) / 16, mt = (p.m + 15) / 16;
+    if (mt == 1 && tiles > 640) {
+        if (p.k < 2048) q4_go<T, MIN, GB, 1, 1, 8, 1, 2>(st, p);
         else if (tiles <= 1280) q4_go<T, MIN, GB, 1, 1, 4, 2, 4>(st, p);
         else q4_go<T, MIN, GB, 1, 1, 8, 1, 4>(st, p);
-    } else if ((tiles + 15) / 16 * ((p.m + 63) / 64) >= 216) q4_go<T, MIN, GB, 4, 2, 8, 1, 1>(st, p);
-    else if ((tiles + 7) / 8 * mt >= 150) q4_go<T, MIN, GB, 2, 1, 8, 1, MS>(st, p);
-    else if ((tiles + 3) / 4 * mt >= 140) q4_go<T, MIN, GB, 2, 1, 4, 2, MS>(st, p);
-    else if ((tiles + 1) / 2 * mt >= 64) q4_go<T, MIN, GB, 2, 1, 2, 4, 1>(st, p);
-    else q4_go<T, MIN, GB, 2, 1, 1, 8, 1>(st, p);
+    } else if (mt > 1 && (tiles + 15) / 16 * ((mt + 3) / 4) >= 216) q4_go<T, MIN, GB, 4, 2, 8, 1, 1>(st, p);
+    else if (mt > 1 && (tiles + 7) / 8 * ((mt + 1) / 2) >= 140) q4_go<T, MIN, GB, 2, 1, 8, 1, MS>(st, p);
+    else if (mt > 1 && (tiles + 3) / 4 * ((mt + 1) / 2) >= 140 * Q4X<T>::PARTS) q4_go<T, MIN, GB, 2, 1, 4, 2, MS>(st, p);
+    else if (mt > 1 && (tiles + 3) / 4 * mt >= 150) q4_go<T, MIN, GB, 1, 1, 4, 2, 1>(st, p);
+    else if (mt > 1 && (tiles + 1) / 2 * mt >= 160) q4_go<T, MIN, GB, 1, 1, 2, 4, 1>(st, p);
+    else q4_go<T, MIN, GB, 1, 1, 1, 8, 1>(st, p);
 }
 template <typename T>
 static void q4_type(hipStream_t st, const Q4P &p) {
