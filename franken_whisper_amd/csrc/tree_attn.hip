@@ -186,6 +186,24 @@ __device__ __forceinline__ bool tree_sees(const TreeP &p, const TreeReq &q, int 
     if (yes && t >= 0) yes = p.words ? p.mask[(int64_t)(q.row0 + i) * p.words + (t >> 6)] >> (t & 63) & 1 : t <= i;
     return yes;
 }
+// The same for 32 keys at once, bit b for key j + b.  One window of the mask row
+// (or a comparison) a row and step, and a bit test a score.
+__device__ __forceinline__ uint32_t tree_window(const TreeP &p, const TreeReq &q, int i, int j, int last) {
+    const int t = j - q.len, left = last - j; // t < 0: cached tokens, which every row sees
+    uint32_t w = ~0u;
+    if (p.words) {
+        const uint64_t *row = p.mask + (int64_t)(q.row0 + i) * p.words;
+        const int at = max(t, 0) >> 6, sh = max(t, 0) & 63;
+        uint64_t v = at < p.words ? row[at] >> sh : 0;
+        if (sh > 32 && at + 1 < p.words) v |= row[at + 1] << (64 - sh);
+        w = (uint32_t)v;
+        if (t < 0) w = t <= -32 ? ~0u : w << -t | ((1u << -t) - 1);
+    } else {
+        const int v = i - t; // bits 0..v
+        w = v < 0 ? 0u : v >= 31 ? ~0u : (2u << v) - 1;
+    }
+    return left <= 0 ? 0u : left >= 32 ? w : w & ((1u << left) - 1);
+}
 // Whether new token i of a request with n of them sees any key.
 __device__ __forceinline__ bool tree_sees_any(const TreeP &p, const TreeReq &q, int i) {
     if (q.len > 0 || !p.words) return true;
@@ -273,12 +291,11 @@ struct Rows {
     }
     // Products of the step at key j to -inf where a row does not see the key.
     __device__ __forceinline__ void mask(const TreeP &p, const TreeReq &rq, int x, int j, int last, f4 (&z)[KT]) const {
-        const int c = (threadIdx.x & 63) >> 4;
+        const uint32_t sees = tree_window(p, rq, node[x], j, last) >> (threadIdx.x >> 2 & 12); // 4 c
 #pragma unroll
         for (int k = 0; k < KT; k++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (!tree_sees(p, rq, node[x], j + k * 16 + 4 * c + i, last)) z[k][i] = -INFINITY;
+            for (int i = 0; i < 4; i++) z[k][i] = sees >> (k * 16 + i) & 1 ? z[k][i] : -INFINITY;
     }
     // Products q . k to weights (in place); what is there already is scaled where the maximum moves.
     __device__ __forceinline__ void weigh(f4 (&z)[RT][KT], float zs) {
@@ -436,6 +453,7 @@ struct Rows {
 struct TreeBlock {
     TreeReq rq;
     int r, kvh, tile, group, total, t0, first, last;
+    int clear; // every row of the block sees every key before this one
     bool whole;
     // false: nothing to do (or done: rows of a bad request)
     template <typename T, int D>
@@ -469,6 +487,7 @@ struct TreeBlock {
         // a chain's rows see no further than the tile's last token
         const int end = p.words ? rq.len + rq.n : rq.len + (min(t0 + p.tile_rows, total) - 1) / group + 1;
         last = whole ? end : min(end, first + chunk);
+        clear = min(last, p.words ? rq.len : rq.len + t0 / group + 1);
         return whole || first < end; // the join reads no part behind the end
     }
     // Where this block's part of row t0 + i goes.
@@ -631,7 +650,7 @@ __global__ void __launch_bounds__(256, 2) k_tree_few(TreeP p) {
                 load();
                 pages(j0 + 8 * KEYS);
             }
-            if (__builtin_expect(j0 + KEYS > min(b.rq.len, last), 0)) rows.mask(p, b.rq, 0, j0, last, z[0]);
+            if (__builtin_expect(j0 + KEYS > b.clear, 0)) rows.mask(p, b.rq, 0, j0, last, z[0]);
             rows.weigh(z, zs);
             rows.template add<VROW>(vt, z);
         }
@@ -744,7 +763,7 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
                 }
             }
             const int j = j0 + wk * KEYS;
-            if (__builtin_expect(j + KEYS > min(b.rq.len, last), 0))
+            if (__builtin_expect(j + KEYS > b.clear, 0))
 #pragma unroll
                 for (int x = 0; x < RT; x++) rows.mask(p, b.rq, x, j, last, z[x]);
             rows.weigh(z, zs);
