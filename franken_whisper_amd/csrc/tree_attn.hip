@@ -13,7 +13,8 @@
 #include "fw_serve.h"
 
 #define TREE_UNITS 1024 // units of a call, at most
-#define TREE_CHUNK 512  // keys of a unit, at least
+#define TREE_CHUNK 128  // keys of a unit, at least
+#define TREE_WHOLE 512  // up to as many keys a request is not cut
 
 struct TreeP {
     int n_req, n_rows, heads, kv_heads, n_pages, width, max_new, max_len, words;
@@ -567,6 +568,8 @@ __device__ __forceinline__ void tree_slow(const TreeP &p, const TreeBlock &b, ch
 // straight to the registers that multiply it, its V tile through LDS of its
 // own, where the transposing read gives each lane the keys of one feature.  The
 // next step's tiles are in flight while a step computes; no barriers.
+// One token of 64 requests over 4,096 cached each (32 heads on 8, 128 wide, bf16): 172 us,
+// 4.66 TB/s.  One request of 225 keys (f32) takes 10 us, four dependent steps a wave.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 2) k_tree_few(TreeP p) {
     typedef Rows<T, D, 1> R;
@@ -669,8 +672,13 @@ __global__ void __launch_bounds__(256, 2) k_tree_few(TreeP p) {
 // through registers into one of two places in LDS: while a step computes, the
 // next step's tiles are on their way from memory and one barrier a step
 // separates the two places.
+// 16 requests x 16 drafted tokens over 32,768 cached each (32 heads on 8, bf16, 64 rows a
+// block): 318 us, 4.87 TB/s, the cache's bytes once.  64 drafted tokens over 131,061
+// (f16, 128 rows a block): 280 us, 490 TFLOP/s of the formula's products, where the vector
+// instructions (weights, their two halves) are active 56% of the time and the matrix
+// units 35%; 32 rows a wave fill the registers.
 template <typename T, int D, int RT, int WR>
-__global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) k_tree_wide(TreeP p) {
+__global__ void __launch_bounds__(256, RT > 1 ? 2 : D == 64 && sizeof(T) == 2 ? 4 : 3) k_tree_wide(TreeP p) {
     typedef Rows<T, D, RT> R;
     constexpr int KT = R::KT, KEYS = R::KEYS, NS = R::NS, WK = 4 / WR, TK = WK * KEYS; // keys of a step
     constexpr int NC = D * (int)sizeof(T) / 16, NL = TK * NC / 256; // 16-byte pieces of a key; of a thread, for K and for V
@@ -848,9 +856,15 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeP p) {
 }
 
 // How a call of these sizes is cut.  Up to 16 rows per K/V head share one tile
-// (k_tree_few); 32, 64 or 128 rows a block above that (k_tree_wide).  Where that
-// gives fewer than 256 blocks the keys are cut into units (tree_units), as many
-// as run at once: 2 to 4 blocks a CU, by the registers and LDS of the kernel.
+// (k_tree_few); 32, 64 or 128 rows a block above that (k_tree_wide).  Where
+// that gives fewer than 256 blocks (one a CU) the keys are cut into units (tree_units),
+// as many as run at once: 2 to 4 blocks a CU, by the registers and LDS of the kernel.
+// Measured on both sides, us, this rule / the other:
+//   24 requests x 8 over 4,096 (192 blocks) cut 90 / 109 whole, 20 x 32 over 3,000 (160)
+//     98 / 119; 32 x 1 over 4,096 (256) whole 92 / 107 cut, 40 x 16 over 2,048 (320) 83 / 91;
+//   units of 128 keys or more, 1 x 1 over 2,048 13.8 / 15.9 (256) / 19.8 (512), 16 x 1 over
+//     1,024 22.6 / 22.7 / 26.0; up to 512 keys whole: 10 x 16 over 440 (20 heads) 12.5 / 16.8
+//     cut, 1 x 8 over 217 10.2 / 13.2: the join is a launch and its latency.
 struct TreeCut {
     int rows, units;
     int64_t tiles;
@@ -864,11 +878,11 @@ static TreeCut tree_cut(int32_t n_req, int32_t n_heads, int32_t n_kv_heads, int3
     t.tiles = (rows + t.rows - 1) / t.rows;
     const int64_t at_once = head_dim == 64 ? (t.rows == 128 ? 768 : TREE_UNITS) : t.rows == 32 || t.rows == 128 ? 512 : 768;
     const int64_t per = std::max<int64_t>(1, (int64_t)n_kv_heads * t.tiles), base = per * n_req;
-    const int64_t most = ((int64_t)max_len + TREE_CHUNK - 1) / TREE_CHUNK * n_req; // units of TREE_CHUNK
+    const int64_t most = max_len <= TREE_WHOLE ? 0 : ((int64_t)max_len + TREE_CHUNK - 1) / TREE_CHUNK * n_req; // units of TREE_CHUNK
     const int64_t units = std::min(at_once / per, most);
     t.units = base >= 256 || units <= n_req ? 0 : (int)units;
     // enough for every smaller call too
-    t.bytes = max_len > TREE_CHUNK ? (uint64_t)std::min(at_once, per * most) * t.rows * (head_dim + 4) * 4 : 0;
+    t.bytes = (uint64_t)std::min(at_once, per * most) * t.rows * (head_dim + 4) * 4;
     return t;
 }
 
