@@ -510,8 +510,9 @@ static void q4_go(hipStream_t st, Q4P p) {
 // carry fewer scale loads and waits but leave more idle at the end of short rows.
 // Measured on both sides, us, the form that runs / the next best of the others:
 //   1..16 rows, up to 640 tiles of 16 outputs: 1 x 5120 x 1280 5.2 / 7.9
-//     k < 2048: 10 x 51866 x 1280 (f32) 18.5 / 32, 1 x 51866 x 1280 13 / 20
-//     up to 1280 tiles: 8 x 14336 x 4096 14.3 / 18.8; above: 16 x 28672 x 8192 44 / 49
+//     k < 2048, from 2048 tiles on 16 waves a block: 10 x 51866 x 1280 (f32) 16.8 / 18.9,
+//     1 x 51866 x 1280 13.0 / 13.4; less, 8 waves: 1 x 12288 x 1280 8.3 / 11.3
+//     up to 1280 tiles: 8 x 14336 x 4096 14.2 / 20.0; above: 16 x 28672 x 8192 37 / 43
 //   more, by how many blocks of 64 rows x 256 outputs, 32 x 128 or 32 x 64 there are,
 //     else of 16 x 64, 16 x 32 or 16 x 16:
 //     1500 x 5120 x 1280 58 / 71 and 700 x 5120 x 1280 28 / 31;
@@ -526,7 +527,8 @@ static void q4_rows(hipStream_t st, const Q4P &p) {
     constexpr int MS = GB == 1 ? 1 : 2;
     const int64_t tiles = (p.n + 15) / 16, mt = (p.m + 15) / 16;
     if (mt == 1 && tiles > 640) {
-        if (p.k < 2048) q4_go<T, MIN, GB, 1, 1, 8, 1, 2>(st, p);
+        if (p.k < 2048 && tiles >= 2048) q4_go<T, MIN, GB, 1, 1, 16, 1, 1>(st, p);
+        else if (p.k < 2048) q4_go<T, MIN, GB, 1, 1, 8, 1, 2>(st, p);
         else if (tiles <= 1280) q4_go<T, MIN, GB, 1, 1, 4, 2, 4>(st, p);
         else q4_go<T, MIN, GB, 1, 1, 8, 1, 4>(st, p);
     } else if (mt > 1 && (tiles + 15) / 16 * ((mt + 3) / 4) >= 216) q4_go<T, MIN, GB, 4, 2, 8, 1, 1>(st, p);

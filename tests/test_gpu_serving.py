@@ -499,7 +499,7 @@ def check_q4(ctx, kind, x, q, scale, mn, b, group, pad=0):
     (130, 200, 160, 32, True, True, "f16", 16), (300, 129, 256, 32, False, True, "f32", 0), (1, 5120, 5120, 32, False, True, "f16", 0),
     (3, 16, 8192, 128, True, False, "f16", 0),
     # one of each form: few and many outputs, short and long rows, several row tiles
-    (10, 10300, 160, 32, True, True, "f16", 0), (9, 11000, 2112, 64, False, True, "f16", 0), (16, 21000, 2176, 128, True, False, "f16", 0),
+    (10, 33000, 192, 32, True, True, "f16", 3), (16, 32777, 1152, 128, False, False, "f32", 0), (10, 10300, 160, 32, True, True, "f16", 0), (9, 11000, 2112, 64, False, True, "f16", 0), (16, 21000, 2176, 128, True, False, "f16", 0),
     (20, 1000, 1056, 32, True, True, "f16", 8), (32, 4100, 288, 32, False, False, "f32", 0), (27, 8300, 384, 128, True, True, "f16", 0),
     (50, 1281, 160, 32, False, True, "f16", 0), (90, 3850, 224, 32, True, True, "f32", 0), (61, 5130, 320, 64, False, False, "f16", 8),
     (130, 5140, 192, 32, True, False, "f16", 0), (1030, 4097, 256, 64, True, True, "f16", 0), (700, 1600, 544, 32, False, True, "f16", 8), (200, 1300, 640, 128, True, True, "f16", 0)])
