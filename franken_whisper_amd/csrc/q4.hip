@@ -149,7 +149,7 @@ __device__ __forceinline__ float q4_one(const Q4P &p, int m, int n) {
 //
 // Bound by the weights' bytes up to about 16 rows: one row through 28,672 x 8,192
 // (bf16, groups of 128 with minimums) takes 29 us, 4.3 TB/s where the same access
-// alone takes 24 (4.9), sixteen rows 40 us: staging x for 224 blocks is the rest.
+// alone takes 24 (4.9), sixteen rows 37 us: staging x for 224 blocks is the rest.
 // With more rows by the instructions around the products (unpacking, scales): 1,500
 // rows through 5,120 x 1,280 (f16, groups of 32 with minimums) take 58 us, 336
 // TFLOP/s; 2,048 through 8,192 x 4,096 (bf16, groups of 128) 255 us, 538 TFLOP/s.
