@@ -305,6 +305,9 @@ def check_attn(ctx, s, **kw):
     ([700, 90], [65, 130], 3, 1, 64, 32, True),            # masks of several words
     ([0, 40], [100, 37], 4, 2, 128, 16, False),            # prompts as chains
     ([2100], [5], 16, 2, 128, 64, True),
+    ([505, 511, 600, 637, 0], [8, 1, 40, 3, 2], 8, 2, 128, 16, True), # the edges of where and how the keys are cut
+    ([504], [8], 4, 4, 64, 16, True), ([505], [8], 4, 4, 64, 16, True), ([1016, 3], [8, 1], 8, 1, 64, 32, True),
+    ([0, 300], [520, 230], 4, 2, 64, 16, False),
     ([1500, 10, 260], [1, 1, 1], 32, 4, 128, 16, False),   # single tokens
 ])
 def test_attention(tctx, kind, lens, n_new, heads, kv, dim, page, tree):
