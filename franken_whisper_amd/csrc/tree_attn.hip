@@ -856,15 +856,21 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeP p) {
 }
 
 // How a call of these sizes is cut.  Up to 16 rows per K/V head share one tile
-// (k_tree_few); 32, 64 or 128 rows a block above that (k_tree_wide).  Where
-// that gives fewer than 256 blocks (one a CU) the keys are cut into units (tree_units),
-// as many as run at once: 2 to 4 blocks a CU, by the registers and LDS of the kernel.
+// (k_tree_few); 32, 64 or 128 rows a block above that (k_tree_wide), 128 only over
+// long caches, where what a block reads matters more than how many blocks there
+// are.  Where that gives fewer than 256 (one a CU) the keys are cut into units
+// (tree_units), as many as run at once: 2 to 4 blocks a CU, by the registers and
+// LDS of the kernel.
 // Measured on both sides, us, this rule / the other:
 //   24 requests x 8 over 4,096 (192 blocks) cut 90 / 109 whole, 20 x 32 over 3,000 (160)
 //     98 / 119; 32 x 1 over 4,096 (256) whole 92 / 107 cut, 40 x 16 over 2,048 (320) 83 / 91;
 //   units of 128 keys or more, 1 x 1 over 2,048 13.8 / 15.9 (256) / 19.8 (512), 16 x 1 over
 //     1,024 22.6 / 22.7 / 26.0; up to 512 keys whole: 10 x 16 over 440 (20 heads) 12.5 / 16.8
-//     cut, 1 x 8 over 217 10.2 / 13.2: the join is a launch and its latency.
+//     cut, 1 x 8 over 217 10.2 / 13.2: the join is a launch and its latency;
+//   64 rows a block over short caches, 10 chains of 224 over 224 (20 heads of 64) 21.3 / 24.0,
+//     64 of them 79 / 93, one of 500 (32 heads on 8, of 128) 21.0 / 26.5, but 10 x 200 over 100
+//     28.3 / 27.0; 128 over long ones, 1 x 64 over 131,061 277 / 310, 8 x 512 over 4,096 401 / 415,
+//     2 x 64 over 32,768 (heads of 64) 86 / 92.
 struct TreeCut {
     int rows, units;
     int64_t tiles;
@@ -874,7 +880,7 @@ static TreeCut tree_cut(int32_t n_req, int32_t n_heads, int32_t n_kv_heads, int3
                         int32_t max_len) {
     TreeCut t;
     const int64_t rows = (int64_t)max_new * (n_heads / n_kv_heads);
-    t.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    t.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 || max_len <= TREE_WHOLE ? 64 : 128;
     t.tiles = (rows + t.rows - 1) / t.rows;
     const int64_t at_once = head_dim == 64 ? (t.rows == 128 ? 768 : TREE_UNITS) : t.rows == 32 || t.rows == 128 ? 512 : 768;
     const int64_t per = std::max<int64_t>(1, (int64_t)n_kv_heads * t.tiles), base = per * n_req;
